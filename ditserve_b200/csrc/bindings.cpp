@@ -742,6 +742,8 @@ void put_peers(const at::Tensor& src, int64_t mask, int64_t dst_off, int64_t ran
 
 }  // namespace
 
+void bind_block_ops(pybind11::module_& m);  // block_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels of ditserve_b200 (tcgen05 GEMM/attention, fused norms, solver step)";
   m.def("gemm", &gemm, "C = epilogue(A @ B^T)");
@@ -770,6 +772,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ring_quant_push", &ring_quant_push, "INT8-quantize this rank's ring K/V chunk into every ring peer's slot");
   m.def("ring_dequant", &ring_dequant, "dequantize one peer's INT8 ring slot into a local bf16 [rows, 3w] buffer");
   m.def("ring_slot_bytes", &ds::ring_slot_bytes, "bytes of one INT8 ring slot");
+  bind_block_ops(m);
   m.attr("FLAG_BYTES") = ds::kFlagBytes;
   m.attr("MAX_PEERS") = ds::kMaxPeers;
   m.attr("CHANNELS") = ds::kChannels;

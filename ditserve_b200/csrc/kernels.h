@@ -240,4 +240,100 @@ void launch_group_flag(const PeerGroup& g, int channel, uint64_t epoch, int flag
 void launch_put_peers(const PeerGroup& g, unsigned mask, const void* src, int64_t bytes, int64_t dst_off,
                       cudaStream_t s);
 
+// ---- operators of a quantised, text-conditioned block ----
+enum ElemType : int { kBF16 = 0, kFP16 = 1, kFP32 = 2 };
+
+// h = round(x + residual) (or x), y = h * rsqrt(mean(h^2) + eps) * w, scale = max(max|y| / 448, 1e-30),
+// q = e4m3(y / scale).  Rows have unit column stride and any row stride (norm_quant.cu).
+struct NormQuantArgs {
+  const void* x = nullptr;
+  int64_t x_stride = 0;
+  const void* residual = nullptr;  // or null
+  int64_t r_stride = 0;
+  void* h = nullptr;               // stored sum; null without a residual.  May alias residual or x.
+  int64_t h_stride = 0;
+  const void* weight = nullptr;    // [dim] in x's type, or null
+  uint8_t* q = nullptr;
+  int64_t q_stride = 0;
+  float* scale = nullptr;          // [rows], scale_stride apart
+  int64_t scale_stride = 1;
+  int64_t rows = 0;
+  int dim = 0;
+  float eps = 1e-6f;
+  int type = kBF16;
+};
+void launch_norm_quant(const NormQuantArgs& a, cudaStream_t stream);
+
+// y = epilogue(sx[m] * sw[n] * sum_k x[m, k] w[n, k] + bias[n]) on e4m3 operands (linear_fp8.cu)
+struct LinearFp8Args {
+  const uint8_t* x = nullptr;  // [M, K], 16-byte aligned rows
+  int64_t ldx = 0;
+  const uint8_t* w = nullptr;  // [N, K], 16-byte aligned rows
+  int64_t ldw = 0;
+  const float* sx = nullptr;   // [M], sx_stride apart
+  int64_t sx_stride = 1;
+  const float* sw = nullptr;   // [N], sw_stride apart
+  int64_t sw_stride = 1;
+  void* y = nullptr;           // [M, N] of out_type
+  int64_t ldy = 0;
+  int M = 0, N = 0, K = 0;
+  int out_type = kBF16;
+  const void* bias = nullptr;      // [N] of out_type, or null
+  const void* residual = nullptr;  // [M, N] of out_type, or null (may alias y)
+  int64_t ldr = 0;
+  const float* gate = nullptr;     // gate[b * gate_stride + n], with a residual only
+  int64_t gate_stride = 0;
+  int rows_per_batch = 0;
+  const int* row_batch = nullptr;
+  int batches = 0;                 // rows of gate: row_batch entries are held below it
+  int gelu = 0;
+  int* status = nullptr;
+};
+void launch_linear_fp8(const LinearFp8Args& a, cudaStream_t stream);
+
+// Rotary positions with several axes on up to two tensors of one token list (rope_axes.cu).
+constexpr int kRopeMaxPairs = 256;
+constexpr int kRopeMaxAxes = 4;
+struct RopeTensor {
+  const void* x = nullptr;
+  int64_t x_stride = 0;
+  void* y = nullptr;
+  int64_t y_stride = 0;
+  int heads = 0;  // 0: absent
+};
+struct RopeAxesArgs {
+  RopeTensor t[2];
+  int64_t rows = 0;
+  int head_dim = 0, pairs = 0;
+  int half = 0;      // pair i = elements (i, i + pairs) instead of (2i, 2i + 1)
+  int inverse = 0;
+  int type = kBF16;
+  const void* pos = nullptr;
+  int64_t pos_rows = 0;   // row r of the tensors takes position row r % pos_rows
+  int64_t pos_stride = 0, axis_stride = 0;
+  int pos_type = 0;       // 0 int64, 1 int32, 2 fp32, 3 fp64
+  double turns[kRopeMaxPairs];  // frequency of each pair / (2 pi)
+  uint8_t axis[kRopeMaxPairs];
+};
+void launch_rope_axes(const RopeAxesArgs& a, cudaStream_t stream);
+
+// Attention of [B, Sq] queries to [B, Sk] encoder states with valid lengths and key masks
+// (cross_attention.cu).  Strides in elements; head h occupies columns [h * head_dim, (h + 1) * head_dim).
+struct CrossAttnArgs {
+  const void* q = nullptr;
+  const void* k = nullptr;
+  const void* v = nullptr;
+  void* o = nullptr;
+  int64_t q_row = 0, q_batch = 0, k_row = 0, k_batch = 0, v_row = 0, v_batch = 0, o_row = 0, o_batch = 0;
+  float* lse = nullptr;  // [B, heads, Sq] contiguous, or null
+  int batch = 0, seq_q = 0, seq_k = 0, heads = 0, heads_kv = 0, head_dim = 0;
+  const int* kv_lens = nullptr;       // [B] valid keys (clamped to [0, Sk]), or null
+  const uint8_t* key_mask = nullptr;  // [B, Sk] non-zero: may be attended to; or null
+  int64_t mask_row = 0, mask_col = 0;
+  float scale = 1.f;
+  int type = kBF16;
+  int* status = nullptr;
+};
+void launch_cross_attention(const CrossAttnArgs& a, cudaStream_t stream);
+
 }  // namespace ds

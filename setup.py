@@ -31,6 +31,11 @@ ext = CUDAExtension(
         os.path.join(CSRC, "noalloc.cu"),
         os.path.join(CSRC, "ring_codec.cu"),
         os.path.join(CSRC, "conv.cu"),
+        os.path.join(CSRC, "block_bindings.cpp"),
+        os.path.join(CSRC, "norm_quant.cu"),
+        os.path.join(CSRC, "linear_fp8.cu"),
+        os.path.join(CSRC, "rope_axes.cu"),
+        os.path.join(CSRC, "cross_attention.cu"),
     ],
     include_dirs=[os.path.join(HERE, CSRC)],
     extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
