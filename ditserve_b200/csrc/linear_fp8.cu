@@ -7,6 +7,7 @@
 #include "kernels.h"
 #include "mma_sync.cuh"
 #include "sm100.cuh"
+#include "tma_host.h"
 
 namespace ds {
 namespace {
@@ -91,6 +92,327 @@ __global__ void __launch_bounds__(32 * kRowWarps) linear_rows_kernel(LinearFp8Ar
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: persistent, warp-specialised tcgen05 product (kind::f8f6f4).  A tile is 128 rows of x per
+// CTA and bn output channels (a multiple of 16 up to 256, a launch parameter).  Warp 0 streams 128-byte
+// k-blocks of both operands with TMA (128-byte swizzle) through a ring of stages, warp 1 issues the
+// products into one of two TMEM accumulators, warps 2..9 scale, finish and store the other.
+// kPair: two CTAs share one 256-row tile (cta_group::2), each staging its rows of x and half of the
+// channels; the leader issues for both, and no operand byte is staged twice in the pair.
+constexpr int kBM = 128, kBK = 128;
+constexpr int kTileThreads = 320;
+constexpr int kMaxBn = 256;
+
+template <bool kPair>
+struct TileCfg {
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kABytes = kBM * kBK;
+  static constexpr int kBBytes = (kPair ? kMaxBn / 2 : kMaxBn) * kBK;
+  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + 1024 + 256;
+};
+
+struct TileShape {
+  int bn, num_m, num_n, num_k;
+  int vec;     // rows of y (and of the residual) start on 32 bytes' worth of 16 elements: vector stores
+  int cvec;    // sw, bias and gate rows allow 16-byte loads
+};
+
+// 16 column parameters at n as floats, the same for every lane
+template <typename P>
+__device__ __forceinline__ void columns16(const P* p, float (&f)[16]) {
+  constexpr int V = kVec16<P>;
+#pragma unroll
+  for (int i = 0; i < 16 / V; ++i) {
+    float t[V];
+    load_vec<P, V>(p + i * V, t);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[i * V + e] = t[e];
+  }
+}
+
+// 32 bytes at once (two 16-bit vectors' worth: a whole sector per lane)
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack2(T(), v[2 * i], v[2 * i + 1]);
+    store32(p, w);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * h + i]);
+      store32(p + 8 * h, w);
+    }
+  }
+}
+
+// 16 accumulator columns of output row m at channel n
+template <typename T>
+__device__ __forceinline__ void finish16(const LinearFp8Args& a, const TileShape& sh, const uint32_t* acc, float sx, int m,
+                                         int n, const float* gate_row) {
+  T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
+  if (sh.vec && sh.cvec && n + 16 <= a.N) {
+    float v[16], c[16];
+    columns16(a.sw + n, c);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(acc[j]) * (sx * c[j]);
+    if (a.bias != nullptr) {
+      columns16(reinterpret_cast<const T*>(a.bias) + n, c);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] += c[j];
+    }
+    if (a.gelu) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          const float u = 0.7978845608028654f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
+          v[j] = v[j] / (1.f + expf(-2.f * u));
+        } else {
+          v[j] = gelu_tanh(v[j]);
+        }
+      }
+    }
+    if (a.residual != nullptr) {
+      if (gate_row != nullptr) {
+        columns16(gate_row + n, c);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] *= c[j];
+      }
+      columns16(reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n, c);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] += c[j];
+    }
+    store16<T>(y, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n + j < a.N)
+        y[j] = from_float<T>(finish<T>(a, __uint_as_float(acc[j]) * (sx * a.sw[(n + j) * a.sw_stride]), m, n + j, gate_row));
+  }
+}
+
+template <typename T, bool kPair>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, LinearFp8Args a,
+                       TileShape sh) {
+  using Cfg = TileCfg<kPair>;
+  constexpr int ST = Cfg::kStages;
+  constexpr int kCtas = kPair ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + ST * Cfg::kABytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sB + ST * Cfg::kBBytes);  // pair: the leader's
+  uint64_t* empty = full + ST;
+  uint64_t* acc_full = empty + ST;
+  uint64_t* acc_empty = acc_full + 2;  // pair: the leader's
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
+  const int tiles = sh.num_m * sh.num_n;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8 * kCtas);  // one arrival per epilogue warp
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    if constexpr (kPair) tmem_alloc_pair<512>(tmem_slot);
+    else tmem_alloc<512>(tmem_slot);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();  // the leader's barriers are ready before the peer signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      const int b_rows = sh.bn / kCtas;
+      const uint32_t bytes = kCtas * (Cfg::kABytes + b_rows * kBK);
+      for (int tile = first; tile < tiles; tile += step) {
+        const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM;
+        const int n0 = (tile % sh.num_n) * sh.bn + rank * b_rows;
+        for (int kb = 0; kb < sh.num_k; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, a.status, 310)) goto producer_done;
+          if constexpr (kPair) {
+            const uint32_t leader = mapa_shared(smem_u32(&full[stage]), 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+            tma_load_2d_pair(sA + stage * Cfg::kABytes, &tmX, kb * kBK, m0, leader);
+            tma_load_2d_pair(sB + stage * Cfg::kBBytes, &tmW, kb * kBK, n0, leader);
+          } else {
+            mbar_arrive_expect_tx(&full[stage], bytes);
+            tma_load_2d(sA + stage * Cfg::kABytes, &tmX, kb * kBK, m0, &full[stage]);
+            tma_load_2d(sB + stage * Cfg::kBBytes, &tmW, kb * kBK, n0, &full[stage]);
+          }
+          if (++stage == ST) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    producer_done:;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = umma_idesc_e4m3(kCtas * kBM, sh.bn);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      for (int tile = first; tile < tiles; tile += step, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, a.status, 311)) goto mma_done;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * kMaxBn;
+        for (int kb = 0; kb < sh.num_k; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag, a.status, 312)) goto mma_done;
+          tc_fence_after();
+          const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * Cfg::kABytes), 16, 1024);
+          const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * Cfg::kBBytes), 16, 1024);
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k) {
+            // 32 bytes onwards inside the swizzle atom: 2 in the address field
+            if constexpr (kPair) umma_e4m3_ss_pair(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            else umma_e4m3_ss(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+          }
+          if constexpr (kPair) umma_commit_pair(&empty[stage]);
+          else umma_commit(&empty[stage]);
+          if (++stage == ST) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if constexpr (kPair) umma_commit_pair(&acc_full[acc]);
+        else umma_commit(&acc_full[acc]);
+      }
+    mma_done:;
+    }
+  } else {
+    const int quarter = warp & 3;             // the TMEM lanes this warp may read
+    const int half = (warp - 2) >> 2;         // the two warps of a quarter take alternate 32-column chunks
+    int local = 0;
+    for (int tile = first; tile < tiles; tile += step, ++local) {
+      const int acc = local & 1;
+      const int m = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32 + lane;
+      const int n0 = (tile % sh.num_n) * sh.bn;
+      const bool row_ok = m < a.M;
+      const float sx = row_ok ? a.sx[m * a.sx_stride] : 0.f;
+      const float* gate_row = row_ok ? gate_of(a, m) : nullptr;
+      if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kMaxBn;
+      for (int c = half * 32; c < sh.bn; c += 64) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        tmem_wait_ld();
+        if (row_ok) {
+          finish16<T>(a, sh, r, sx, m, n0 + c, gate_row);
+          if (c + 16 < sh.bn) finish16<T>(a, sh, r + 16, sx, m, n0 + c + 16, gate_row);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+        else mbar_arrive(&acc_empty[acc]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) {
+    // copies that may still be in flight get time to land
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  if constexpr (kPair) cluster_sync_all();  // no CTA leaves while its partner may still address its memory
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (kPair) tmem_dealloc_pair<512>(tmem_base);
+    else tmem_dealloc<512>(tmem_base);
+  }
+}
+
+template <typename T, bool kPair>
+void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
+  using Cfg = TileCfg<kPair>;
+  constexpr int kCtas = kPair ? 2 : 1;
+  auto kern = linear_tile_kernel<T, kPair>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+  const CUtensorMap tmX = make_tmap_u8_2d(a.x, a.M, a.K, a.ldx, kBM);
+  const CUtensorMap tmW = make_tmap_u8_2d(a.w, a.N, a.K, a.ldw, bn / kCtas);
+  auto at = [](const void* p, int64_t bytes, int n) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % n == 0 && bytes % n == 0);
+  };
+  const int64_t e = sizeof(T);
+  TileShape sh;
+  sh.bn = bn;
+  sh.num_m = (a.M + kCtas * kBM - 1) / (kCtas * kBM);
+  sh.num_n = (a.N + bn - 1) / bn;
+  sh.num_k = (a.K + kBK - 1) / kBK;
+  sh.vec = at(a.y, a.ldy * e, 32) && at(a.residual, a.ldr * e, 16);
+  sh.cvec = a.sw_stride == 1 && at(a.sw, 0, 16) && at(a.bias, 0, 16) && at(a.gate, a.gate_stride * 4, 16);
+  const int64_t tiles = static_cast<int64_t>(sh.num_m) * sh.num_n;
+  if (tiles > 0x3fffffff) throw std::runtime_error("linear_fp8: too many tiles");
+  const int slots = device_sm_count() / kCtas;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kCtas * static_cast<unsigned>(tiles < slots ? tiles : slots));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, tmX, tmW, a, sh);
+}
+
+// Width of the tiles: the multiple of 16 whose rounds over the SMs cost least, a round being as long as
+// its tile is wide plus a fixed part (a narrow tile stages as many rows of x as a wide one).
+int pick_bn(int64_t num_m, int N, int slots) {
+  int best = kMaxBn;
+  int64_t cost = INT64_MAX;
+  for (int bn = kMaxBn; bn >= 32; bn -= 16) {
+    const int64_t tiles = num_m * ((N + bn - 1) / bn);
+    const int64_t c = (tiles + slots - 1) / slots * (bn + 48);
+    if (c < cost) {
+      cost = c;
+      best = bn;
+    }
+  }
+  return best;
+}
+
 template <typename T>
 void launch_type(const LinearFp8Args& a, cudaStream_t s) {
   const unsigned gx = (a.N + 15) / 16;
@@ -98,8 +420,12 @@ void launch_type(const LinearFp8Args& a, cudaStream_t s) {
     linear_rows_kernel<T, 1><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
   } else if (a.M <= 16) {
     linear_rows_kernel<T, 2><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
+  } else if (a.M <= 32) {
+    linear_rows_kernel<T, 4><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
   } else {
-    linear_rows_kernel<T, 4><<<dim3(gx, (a.M + 31) / 32), 32 * kRowWarps, 0, s>>>(a);
+    const int sms = device_sm_count();
+    if (a.M <= kBM) launch_tiles<T, false>(a, pick_bn(1, a.N, sms), s);
+    else launch_tiles<T, true>(a, pick_bn((a.M + 2 * kBM - 1) / (2 * kBM), a.N, sms / 2), s);
   }
 }
 

@@ -51,6 +51,26 @@ inline CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t rows, uint64_t c
   return map;
 }
 
+// A row-major [rows, cols] view of bytes in boxes of box_rows x 128 (one swizzle atom wide).  The
+// base and the row stride are multiples of 16 bytes; cols may be any number (the rest of a box
+// behind it reads as zero).
+inline CUtensorMap make_tmap_u8_2d(const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride,
+                                   uint32_t box_rows) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) throw std::runtime_error("TMA base must be 16-byte aligned");
+  if (row_stride % 16 != 0) throw std::runtime_error("TMA row stride must be a multiple of 16 bytes");
+  if (box_rows == 0 || box_rows > 256) throw std::runtime_error("TMA box must be at most 256 rows");
+  CUtensorMap map;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {row_stride};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t elem_strides[2] = {1, 1};
+  CUresult r = encode_tiled_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                                 elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return map;
+}
+
 inline int device_sm_count() {
   int dev = 0, n = 0;
   cudaGetDevice(&dev);
