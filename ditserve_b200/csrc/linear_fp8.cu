@@ -103,107 +103,82 @@ constexpr int kBM = 128, kBK = 128;
 constexpr int kTileThreads = 320;
 constexpr int kMaxBn = 256;
 
+// An epilogue warp stages 32 rows x 64 bytes of y at a time in one of three buffers, from which a tile
+// store takes them (whole sectors; a lane's own stores of its row reached 1.3 TB/s), and keeps the scales
+// and biases of its columns of the tile.
+constexpr int kOutBuffers = 3, kOutBytes = 32 * 64, kColBytes = 2 * (kMaxBn / 2) * 4;
+
 template <bool kPair>
 struct TileCfg {
-  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStages = kPair ? 5 : 3;
   static constexpr int kABytes = kBM * kBK;
   static constexpr int kBBytes = (kPair ? kMaxBn / 2 : kMaxBn) * kBK;
-  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + 1024 + 256;
+  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + 8 * (kOutBuffers * kOutBytes + kColBytes) + 1024 + 256;
 };
 
 struct TileShape {
   int bn, num_m, num_n, num_k;
-  int vec;     // rows of y (and of the residual) start on 32 bytes' worth of 16 elements: vector stores
-  int cvec;    // sw, bias and gate rows allow 16-byte loads
+  int fast;  // y and the residual have rows on 16 bytes, gate rows too: tile stores
 };
 
-// 16 column parameters at n as floats, the same for every lane
-template <typename P>
-__device__ __forceinline__ void columns16(const P* p, float (&f)[16]) {
-  constexpr int V = kVec16<P>;
+// kU accumulator columns of output row m from channel n on: scale, bias, activation, gate, residual.
+// cols holds the columns' scales, then (at kMaxBn / 2) their biases.
+template <typename T, int kU>
+__device__ __forceinline__ void finish_unit(const LinearFp8Args& a, const uint32_t (&acc)[kU], const float* cols, float sx,
+                                            int m, int n, bool row_ok, const float* gate_row, float (&v)[kU]) {
 #pragma unroll
-  for (int i = 0; i < 16 / V; ++i) {
-    float t[V];
-    load_vec<P, V>(p + i * V, t);
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[i * V + e] = t[e];
+  for (int j = 0; j < kU; j += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(cols + j);
+    const float4 b = *reinterpret_cast<const float4*>(cols + kMaxBn / 2 + j);
+    v[j] = fmaf(__uint_as_float(acc[j]), sx * s.x, b.x);
+    v[j + 1] = fmaf(__uint_as_float(acc[j + 1]), sx * s.y, b.y);
+    v[j + 2] = fmaf(__uint_as_float(acc[j + 2]), sx * s.z, b.z);
+    v[j + 3] = fmaf(__uint_as_float(acc[j + 3]), sx * s.w, b.w);
   }
-}
-
-// 32 bytes at once (two 16-bit vectors' worth: a whole sector per lane)
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
-
-template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
-  if constexpr (sizeof(T) == 2) {
-    uint32_t w[8];
+  if (a.gelu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack2(T(), v[2 * i], v[2 * i + 1]);
-    store32(p, w);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * h + i]);
-      store32(p + 8 * h, w);
+    for (int j = 0; j < kU; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        const float u = 0.7978845608028654f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
+        v[j] = v[j] / (1.f + expf(-2.f * u));
+      } else {
+        v[j] = gelu_tanh(v[j]);
+      }
     }
   }
-}
-
-// 16 accumulator columns of output row m at channel n
-template <typename T>
-__device__ __forceinline__ void finish16(const LinearFp8Args& a, const TileShape& sh, const uint32_t* acc, float sx, int m,
-                                         int n, const float* gate_row) {
-  T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
-  if (sh.vec && sh.cvec && n + 16 <= a.N) {
-    float v[16], c[16];
-    columns16(a.sw + n, c);
+  if (a.residual != nullptr && row_ok) {
+    constexpr int V = kVec16<T>;
+    const T* r = reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(acc[j]) * (sx * c[j]);
-    if (a.bias != nullptr) {
-      columns16(reinterpret_cast<const T*>(a.bias) + n, c);
+    for (int j = 0; j < kU; j += V) {
+      if (n + j + V <= a.N) {
+        float f[V];
+        load_vec<T, V>(r + j, f);
+        if (gate_row != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] += c[j];
-    }
-    if (a.gelu) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if constexpr (sizeof(T) == 4) {
-          const float u = 0.7978845608028654f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
-          v[j] = v[j] / (1.f + expf(-2.f * u));
-        } else {
-          v[j] = gelu_tanh(v[j]);
+          for (int e = 0; e < V; e += 4) {
+            const float4 g = *reinterpret_cast<const float4*>(gate_row + n + j + e);
+            v[j + e] *= g.x;
+            v[j + e + 1] *= g.y;
+            v[j + e + 2] *= g.z;
+            v[j + e + 3] *= g.w;
+          }
         }
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[j + e] += f[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (n + j + e < a.N) v[j + e] = fmaf(v[j + e], gate_row != nullptr ? gate_row[n + j + e] : 1.f, to_float(r[j + e]));
       }
     }
-    if (a.residual != nullptr) {
-      if (gate_row != nullptr) {
-        columns16(gate_row + n, c);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] *= c[j];
-      }
-      columns16(reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n, c);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] += c[j];
-    }
-    store16<T>(y, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (n + j < a.N)
-        y[j] = from_float<T>(finish<T>(a, __uint_as_float(acc[j]) * (sx * a.sw[(n + j) * a.sw_stride]), m, n + j, gate_row));
   }
 }
 
 template <typename T, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, LinearFp8Args a,
-                       TileShape sh) {
+    linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmY, LinearFp8Args a, TileShape sh) {
   using Cfg = TileCfg<kPair>;
   constexpr int ST = Cfg::kStages;
   constexpr int kCtas = kPair ? 2 : 1;
@@ -211,7 +186,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + ST * Cfg::kABytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sB + ST * Cfg::kBBytes);  // pair: the leader's
+  uint8_t* sOut = sB + ST * Cfg::kBBytes;
+  float* sCol = reinterpret_cast<float*>(sOut + 8 * kOutBuffers * kOutBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sCol + 8 * kColBytes / 4);  // pair: the leader's
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + 2;  // pair: the leader's
@@ -312,26 +289,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mma_done:;
     }
   } else {
+    constexpr int kU = 64 / sizeof(T);        // columns of a unit (64 bytes of y)
     const int quarter = warp & 3;             // the TMEM lanes this warp may read
-    const int half = (warp - 2) >> 2;         // the two warps of a quarter take alternate 32-column chunks
-    int local = 0;
+    const int half = (warp - 2) >> 2;         // the two warps of a quarter take alternate units
+    uint8_t* out = sOut + (warp - 2) * kOutBuffers * kOutBytes;
+    float* cols = sCol + (warp - 2) * (kColBytes / 4);
+    int local = 0, buf = 0;
     for (int tile = first; tile < tiles; tile += step, ++local) {
       const int acc = local & 1;
-      const int m = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32 + lane;
+      const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32;
+      const int m = m0 + lane;
       const int n0 = (tile % sh.num_n) * sh.bn;
       const bool row_ok = m < a.M;
       const float sx = row_ok ? a.sx[m * a.sx_stride] : 0.f;
       const float* gate_row = row_ok ? gate_of(a, m) : nullptr;
+#pragma unroll
+      for (int i = lane; i < kMaxBn / 2; i += 32) {
+        const int c = (2 * (i / kU) + half) * kU + i % kU, n = n0 + c;  // this warp's i-th column of the tile
+        const bool on = c < sh.bn && n < a.N;
+        cols[i] = on ? a.sw[n * a.sw_stride] : 0.f;
+        cols[kMaxBn / 2 + i] = on && a.bias != nullptr ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
+      }
+      __syncwarp();
       if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kMaxBn;
-      for (int c = half * 32; c < sh.bn; c += 64) {
-        uint32_t r[32];
-        tmem_ld32(taddr + c, r);
+#pragma unroll 1
+      for (int c = half * kU; c < sh.bn; c += 2 * kU) {
+        uint32_t r[kU];
+        if constexpr (kU == 32) tmem_ld32(taddr + c, r);
+        else tmem_ld16(taddr + c, r);
         tmem_wait_ld();
-        if (row_ok) {
-          finish16<T>(a, sh, r, sx, m, n0 + c, gate_row);
-          if (c + 16 < sh.bn) finish16<T>(a, sh, r + 16, sx, m, n0 + c + 16, gate_row);
+        float v[kU];
+        const int n = n0 + c;
+        if (sh.fast && c + kU <= sh.bn) {
+          finish_unit<T, kU>(a, r, cols + c / 2 - half * (kU / 2), sx, m, n, row_ok, gate_row, v);
+          if (lane == 0) tma_store_wait_read<kOutBuffers - 1>();  // the buffer's last store has read it
+          __syncwarp();
+          uint8_t* b = out + buf * kOutBytes;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)  // 16-byte pieces in the 64-byte swizzle's places
+            store_vec<T, kVec16<T>>(reinterpret_cast<T*>(b + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)),
+                                    *reinterpret_cast<const float(*)[kVec16<T>]>(&v[q * kVec16<T>]));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (m0 < a.M && n < a.N) tma_store_2d(&tmY, n, m0, b);
+            tma_store_commit();
+          }
+          buf = buf + 1 == kOutBuffers ? 0 : buf + 1;
+        } else if (row_ok) {
+          // rows off 16 bytes, and the 16 columns that a tile of odd width leaves behind its last unit
+          const int end = min(min(kU, sh.bn - c), a.N - n);
+          T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
+#pragma unroll
+          for (int j = 0; j < kU; ++j)
+            if (j < end)
+              y[j] = from_float<T>(
+                  finish<T>(a, __uint_as_float(r[j]) * (sx * a.sw[(n + j) * a.sw_stride]), m, n + j, gate_row));
         }
       }
       tc_fence_before();
@@ -341,6 +356,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         else mbar_arrive(&acc_empty[acc]);
       }
     }
+    if (lane == 0) tma_store_wait_all();
   }
 
   tc_fence_before();
@@ -377,8 +393,9 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   sh.num_m = (a.M + kCtas * kBM - 1) / (kCtas * kBM);
   sh.num_n = (a.N + bn - 1) / bn;
   sh.num_k = (a.K + kBK - 1) / kBK;
-  sh.vec = at(a.y, a.ldy * e, 32) && at(a.residual, a.ldr * e, 16);
-  sh.cvec = a.sw_stride == 1 && at(a.sw, 0, 16) && at(a.bias, 0, 16) && at(a.gate, a.gate_stride * 4, 16);
+  sh.fast = at(a.y, a.ldy * e, 16) && at(a.residual, a.ldr * e, 16) && at(a.gate, a.gate_stride * 4, 16);
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  const CUtensorMap tmY = sh.fast ? make_tmap_out_2d(a.y, type, sizeof(T), a.M, a.N, a.ldy, 32) : tmX;
   const int64_t tiles = static_cast<int64_t>(sh.num_m) * sh.num_n;
   if (tiles > 0x3fffffff) throw std::runtime_error("linear_fp8: too many tiles");
   const int slots = device_sm_count() / kCtas;
@@ -394,7 +411,7 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, tmX, tmW, a, sh);
+  cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, a, sh);
 }
 
 // Width of the tiles: the multiple of 16 whose rounds over the SMs cost least, a round being as long as

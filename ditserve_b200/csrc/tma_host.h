@@ -71,6 +71,21 @@ inline CUtensorMap make_tmap_u8_2d(const void* base, uint64_t rows, uint64_t col
   return map;
 }
 
+// A row-major output view of 2- or 4-byte elements in boxes of box_rows x 64 bytes (64-byte swizzle).
+inline CUtensorMap make_tmap_out_2d(void* base, CUtensorMapDataType type, int elem, uint64_t rows, uint64_t cols,
+                                    uint64_t row_stride, uint32_t box_rows) {
+  CUtensorMap map;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {row_stride * elem};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(64 / elem), box_rows};
+  cuuint32_t elem_strides[2] = {1, 1};
+  CUresult r = encode_tiled_fn()(&map, type, 2, base, dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return map;
+}
+
 inline int device_sm_count() {
   int dev = 0, n = 0;
   cudaGetDevice(&dev);
