@@ -96,24 +96,25 @@ __global__ void __launch_bounds__(32 * kRowWarps) linear_rows_kernel(LinearFp8Ar
 // Many rows: persistent, warp-specialised tcgen05 product (kind::f8f6f4).  A tile is 128 rows of x per
 // CTA and bn output channels (a multiple of 16 up to 256, a launch parameter).  Warp 0 streams 128-byte
 // k-blocks of both operands with TMA (128-byte swizzle) through a ring of stages, warp 1 issues the
-// products into one of two TMEM accumulators, warps 2..9 scale, finish and store the other.
+// products into one of two TMEM accumulators, warps 2..17 scale, finish and store the other.
 // kPair: two CTAs share one 256-row tile (cta_group::2), each staging its rows of x and half of the
 // channels; the leader issues for both, and no operand byte is staged twice in the pair.
 constexpr int kBM = 128, kBK = 128;
-constexpr int kTileThreads = 320;
+constexpr int kEpiWarps = 16, kEpiParts = kEpiWarps / 4;
+constexpr int kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxBn = 256;
 
-// An epilogue warp stages 32 rows x 64 bytes of y at a time in one of three buffers, from which a tile
+// An epilogue warp stages 32 rows x 64 bytes of y at a time in one of two buffers, from which a tile
 // store takes them (whole sectors; a lane's own stores of its row reached 1.3 TB/s), and keeps the scales
-// and biases of its columns of the tile.
-constexpr int kOutBuffers = 3, kOutBytes = 32 * 64, kColBytes = 2 * (kMaxBn / 2) * 4;
+// and biases of its quarter of the tile's columns.
+constexpr int kOutBuffers = 2, kOutBytes = 32 * 64, kCols = kMaxBn / kEpiParts, kColBytes = 2 * kCols * 4;
 
 template <bool kPair>
 struct TileCfg {
-  static constexpr int kStages = kPair ? 5 : 3;
+  static constexpr int kStages = kPair ? 4 : 3;
   static constexpr int kABytes = kBM * kBK;
   static constexpr int kBBytes = (kPair ? kMaxBn / 2 : kMaxBn) * kBK;
-  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + 8 * (kOutBuffers * kOutBytes + kColBytes) + 1024 + 256;
+  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + kEpiWarps * (kOutBuffers * kOutBytes + kColBytes) + 1024 + 256;
 };
 
 struct TileShape {
@@ -121,29 +122,58 @@ struct TileShape {
   int fast;  // y and the residual have rows on 16 bytes, gate rows too: tile stores
 };
 
+// two floats at once on the packed datapath
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+
+// gelu_tanh of two values: u = x (k0 + k0 k1 x^2), x / 2 + x / 2 tanh u
+__device__ __forceinline__ float2 gelu2(float2 x) {
+  constexpr float k0 = 0.7978845608028654f, k01 = 0.7978845608028654f * 0.044715f;
+  const float2 u = mul2(x, fma2(mul2(x, x), make_float2(k01, k01), make_float2(k0, k0)));
+  const float2 h = mul2(x, make_float2(0.5f, 0.5f));
+  return fma2(h, make_float2(tanh_approx(u.x), tanh_approx(u.y)), h);
+}
+
 // kU accumulator columns of output row m from channel n on: scale, bias, activation, gate, residual.
-// cols holds the columns' scales, then (at kMaxBn / 2) their biases.
+// cols holds the columns' scales, then (at kCols) their biases.
 template <typename T, int kU>
 __device__ __forceinline__ void finish_unit(const LinearFp8Args& a, const uint32_t (&acc)[kU], const float* cols, float sx,
                                             int m, int n, bool row_ok, const float* gate_row, float (&v)[kU]) {
+  const float2 sx2 = make_float2(sx, sx);
 #pragma unroll
   for (int j = 0; j < kU; j += 4) {
     const float4 s = *reinterpret_cast<const float4*>(cols + j);
-    const float4 b = *reinterpret_cast<const float4*>(cols + kMaxBn / 2 + j);
-    v[j] = fmaf(__uint_as_float(acc[j]), sx * s.x, b.x);
-    v[j + 1] = fmaf(__uint_as_float(acc[j + 1]), sx * s.y, b.y);
-    v[j + 2] = fmaf(__uint_as_float(acc[j + 2]), sx * s.z, b.z);
-    v[j + 3] = fmaf(__uint_as_float(acc[j + 3]), sx * s.w, b.w);
+    const float4 b = *reinterpret_cast<const float4*>(cols + kCols + j);
+    float2 x = fma2(make_float2(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1])), mul2(sx2, make_float2(s.x, s.y)),
+                    make_float2(b.x, b.y));
+    float2 y = fma2(make_float2(__uint_as_float(acc[j + 2]), __uint_as_float(acc[j + 3])),
+                    mul2(sx2, make_float2(s.z, s.w)), make_float2(b.z, b.w));
+    if (sizeof(T) == 2 && a.gelu) {
+      x = gelu2(x);
+      y = gelu2(y);
+    }
+    v[j] = x.x;
+    v[j + 1] = x.y;
+    v[j + 2] = y.x;
+    v[j + 3] = y.y;
   }
-  if (a.gelu) {
+  if (sizeof(T) == 4 && a.gelu) {
 #pragma unroll
     for (int j = 0; j < kU; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        const float u = 0.7978845608028654f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
-        v[j] = v[j] / (1.f + expf(-2.f * u));
-      } else {
-        v[j] = gelu_tanh(v[j]);
-      }
+      const float u = 0.7978845608028654f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
+      v[j] = v[j] / (1.f + expf(-2.f * u));
     }
   }
   if (a.residual != nullptr && row_ok) {
@@ -187,8 +217,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* sA = smem;
   uint8_t* sB = smem + ST * Cfg::kABytes;
   uint8_t* sOut = sB + ST * Cfg::kBBytes;
-  float* sCol = reinterpret_cast<float*>(sOut + 8 * kOutBuffers * kOutBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sCol + 8 * kColBytes / 4);  // pair: the leader's
+  float* sCol = reinterpret_cast<float*>(sOut + kEpiWarps * kOutBuffers * kOutBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sCol + kEpiWarps * kColBytes / 4);  // pair: the leader's
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + 2;  // pair: the leader's
@@ -207,7 +237,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 8 * kCtas);  // one arrival per epilogue warp
+      mbar_init(&acc_empty[i], kEpiWarps * kCtas);  // one arrival per epilogue warp
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -291,9 +321,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else {
     constexpr int kU = 64 / sizeof(T);        // columns of a unit (64 bytes of y)
     const int quarter = warp & 3;             // the TMEM lanes this warp may read
-    const int half = (warp - 2) >> 2;         // the two warps of a quarter take alternate units
+    const int part = (warp - 2) >> 2;         // the warps of a quarter take turns at the units
     uint8_t* out = sOut + (warp - 2) * kOutBuffers * kOutBytes;
     float* cols = sCol + (warp - 2) * (kColBytes / 4);
+    // a tile's parameters of this lane: its row's scale, its two columns' scales and biases.  They are
+    // fetched one tile ahead
+    float p_sx = 0.f, p_sw[kCols / 32] = {}, p_b[kCols / 32] = {};
+    auto fetch = [&](int tile) {
+      if (tile >= tiles) return;
+      const int m = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32 + lane;
+      p_sx = m < a.M ? a.sx[m * a.sx_stride] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const int k = i * 32 + lane;                                       // this warp's k-th column of the tile
+        const int c = (kEpiParts * (k / kU) + part) * kU + k % kU, n = (tile % sh.num_n) * sh.bn + c;
+        const bool on = c < sh.bn && n < a.N;
+        p_sw[i] = on ? a.sw[n * a.sw_stride] : 0.f;
+        p_b[i] = on && a.bias != nullptr ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
+      }
+    };
+    // the accumulator goes back as soon as this warp's last columns are in registers
+    auto hand_back = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+        else mbar_arrive(&acc_empty[acc]);
+      }
+    };
+    fetch(first);
     int local = 0, buf = 0;
     for (int tile = first; tile < tiles; tile += step, ++local) {
       const int acc = local & 1;
@@ -301,29 +357,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int m = m0 + lane;
       const int n0 = (tile % sh.num_n) * sh.bn;
       const bool row_ok = m < a.M;
-      const float sx = row_ok ? a.sx[m * a.sx_stride] : 0.f;
+      const float sx = p_sx;
       const float* gate_row = row_ok ? gate_of(a, m) : nullptr;
 #pragma unroll
-      for (int i = lane; i < kMaxBn / 2; i += 32) {
-        const int c = (2 * (i / kU) + half) * kU + i % kU, n = n0 + c;  // this warp's i-th column of the tile
-        const bool on = c < sh.bn && n < a.N;
-        cols[i] = on ? a.sw[n * a.sw_stride] : 0.f;
-        cols[kMaxBn / 2 + i] = on && a.bias != nullptr ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
+      for (int i = 0; i < kCols / 32; ++i) {
+        cols[i * 32 + lane] = p_sw[i];
+        cols[kCols + i * 32 + lane] = p_b[i];
       }
+      fetch(tile + step);
       __syncwarp();
       if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kMaxBn;
 #pragma unroll 1
-      for (int c = half * kU; c < sh.bn; c += 2 * kU) {
+      for (int c = part * kU; c < sh.bn; c += kEpiParts * kU) {
         uint32_t r[kU];
         if constexpr (kU == 32) tmem_ld32(taddr + c, r);
         else tmem_ld16(taddr + c, r);
         tmem_wait_ld();
+        if (c + kEpiParts * kU >= sh.bn) hand_back(acc);
         float v[kU];
         const int n = n0 + c;
         if (sh.fast && c + kU <= sh.bn) {
-          finish_unit<T, kU>(a, r, cols + c / 2 - half * (kU / 2), sx, m, n, row_ok, gate_row, v);
+          finish_unit<T, kU>(a, r, cols + (c / kU / kEpiParts) * kU, sx, m, n, row_ok, gate_row, v);
           if (lane == 0) tma_store_wait_read<kOutBuffers - 1>();  // the buffer's last store has read it
           __syncwarp();
           uint8_t* b = out + buf * kOutBytes;
@@ -349,12 +405,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                   finish<T>(a, __uint_as_float(r[j]) * (sx * a.sw[(n + j) * a.sw_stride]), m, n + j, gate_row));
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
-        else mbar_arrive(&acc_empty[acc]);
-      }
+      if (part * kU >= sh.bn) hand_back(acc);  // a narrow tile has no unit for this warp
     }
     if (lane == 0) tma_store_wait_all();
   }
