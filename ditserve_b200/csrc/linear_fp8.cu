@@ -3,6 +3,8 @@
 //   y[m, n] = epilogue(sx[m] * sw[n] * sum_k x[m, k] * w[n, k] + b[n])
 //
 // x and w are e4m3 with one fp32 scale a row (a token, an output channel); sums are fp32.
+#include <algorithm>
+
 #include "elem.cuh"
 #include "kernels.h"
 #include "mma_sync.cuh"
@@ -104,21 +106,18 @@ constexpr int kEpiWarps = 16, kEpiParts = kEpiWarps / 4;
 constexpr int kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxBn = 256;
 
-// An epilogue warp stages 32 rows x 64 bytes of y at a time in one of two buffers, from which a tile
-// store takes them (whole sectors; a lane's own stores of its row reached 1.3 TB/s), and keeps the scales
-// and biases of its quarter of the tile's columns.
-constexpr int kOutBuffers = 2, kOutBytes = 32 * 64, kCols = kMaxBn / kEpiParts, kColBytes = 2 * kCols * 4;
-
-template <bool kPair>
-struct TileCfg {
-  static constexpr int kStages = kPair ? 4 : 3;
-  static constexpr int kABytes = kBM * kBK;
-  static constexpr int kBBytes = (kPair ? kMaxBn / 2 : kMaxBn) * kBK;
-  static constexpr int kSmemBytes = kStages * (kABytes + kBBytes) + kEpiWarps * (kOutBuffers * kOutBytes + kColBytes) + 1024 + 256;
-};
+// An epilogue warp stages 32 rows x 64 bytes of y at a time, from which a tile store takes them (whole
+// sectors), and keeps the scales and biases of its quarter of the tile's columns.  What shared memory is
+// left holds as many k-blocks as fit (at most kMaxStages): a stage's round trip takes about 2000 cycles,
+// its products 512 at most, so a narrow tile needs the deeper ring.
+constexpr int kOutBytes = 32 * 64, kCols = kMaxBn / kEpiParts, kColBytes = 2 * kCols * 4;
+constexpr int kMaxStages = 10;
+constexpr int kSmemBytes = 227 * 1024;
+constexpr int kSmemFixed = kEpiWarps * (kOutBytes + kColBytes) + 1024 /*align*/ + 256 /*barriers*/;
 
 struct TileShape {
   int bn, num_m, num_n, num_k;
+  int stages, stage_bytes;
   int fast;  // y and the residual have rows on 16 bytes, gate rows too: tile stores
 };
 
@@ -209,16 +208,17 @@ template <typename T, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ CUtensorMap tmY, LinearFp8Args a, TileShape sh) {
-  using Cfg = TileCfg<kPair>;
-  constexpr int ST = Cfg::kStages;
   constexpr int kCtas = kPair ? 2 : 1;
+  const int ST = sh.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + ST * Cfg::kABytes;
-  uint8_t* sOut = sB + ST * Cfg::kBBytes;
-  float* sCol = reinterpret_cast<float*>(sOut + kEpiWarps * kOutBuffers * kOutBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sCol + kEpiWarps * kColBytes / 4);  // pair: the leader's
+  // barriers, staged outputs and columns first (1024-byte aligned as a whole), then the ring: a stage is
+  // 128 rows of x and this CTA's channels
+  uint8_t* sOut = smem;
+  float* sCol = reinterpret_cast<float*>(sOut + kEpiWarps * kOutBytes);
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sCol) + kEpiWarps * kColBytes;
+  constexpr int kABytes = kBM * kBK;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + ST * sh.stage_bytes);  // pair: the leader's
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + 2;  // pair: the leader's
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       const int b_rows = sh.bn / kCtas;
-      const uint32_t bytes = kCtas * (Cfg::kABytes + b_rows * kBK);
+      const uint32_t bytes = kCtas * sh.stage_bytes;
       for (int tile = first; tile < tiles; tile += step) {
         const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM;
         const int n0 = (tile % sh.num_n) * sh.bn + rank * b_rows;
@@ -270,12 +270,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if constexpr (kPair) {
             const uint32_t leader = mapa_shared(smem_u32(&full[stage]), 0);
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-            tma_load_2d_pair(sA + stage * Cfg::kABytes, &tmX, kb * kBK, m0, leader);
-            tma_load_2d_pair(sB + stage * Cfg::kBBytes, &tmW, kb * kBK, n0, leader);
+            tma_load_2d_pair(ring + stage * sh.stage_bytes, &tmX, kb * kBK, m0, leader);
+            tma_load_2d_pair(ring + stage * sh.stage_bytes + kABytes, &tmW, kb * kBK, n0, leader);
           } else {
             mbar_arrive_expect_tx(&full[stage], bytes);
-            tma_load_2d(sA + stage * Cfg::kABytes, &tmX, kb * kBK, m0, &full[stage]);
-            tma_load_2d(sB + stage * Cfg::kBBytes, &tmW, kb * kBK, n0, &full[stage]);
+            tma_load_2d(ring + stage * sh.stage_bytes, &tmX, kb * kBK, m0, &full[stage]);
+            tma_load_2d(ring + stage * sh.stage_bytes + kABytes, &tmW, kb * kBK, n0, &full[stage]);
           }
           if (++stage == ST) {
             stage = 0;
@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int kb = 0; kb < sh.num_k; ++kb) {
           if (!mbar_wait(&full[stage], phase, abort_flag, a.status, 312)) goto mma_done;
           tc_fence_after();
-          const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * Cfg::kABytes), 16, 1024);
-          const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * Cfg::kBBytes), 16, 1024);
+          const uint64_t da = umma_desc_sw128(smem_u32(ring + stage * sh.stage_bytes), 16, 1024);
+          const uint64_t db = umma_desc_sw128(smem_u32(ring + stage * sh.stage_bytes + kABytes), 16, 1024);
 #pragma unroll
           for (int k = 0; k < kBK / 32; ++k) {
             // 32 bytes onwards inside the swizzle atom: 2 in the address field
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int kU = 64 / sizeof(T);        // columns of a unit (64 bytes of y)
     const int quarter = warp & 3;             // the TMEM lanes this warp may read
     const int part = (warp - 2) >> 2;         // the warps of a quarter take turns at the units
-    uint8_t* out = sOut + (warp - 2) * kOutBuffers * kOutBytes;
+    uint8_t* b = sOut + (warp - 2) * kOutBytes;
     float* cols = sCol + (warp - 2) * (kColBytes / 4);
     // a tile's parameters of this lane: its row's scale, its two columns' scales and biases.  They are
     // fetched one tile ahead
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     };
     fetch(first);
-    int local = 0, buf = 0;
+    int local = 0;
     for (int tile = first; tile < tiles; tile += step, ++local) {
       const int acc = local & 1;
       const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32;
@@ -380,9 +380,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int n = n0 + c;
         if (sh.fast && c + kU <= sh.bn) {
           finish_unit<T, kU>(a, r, cols + (c / kU / kEpiParts) * kU, sx, m, n, row_ok, gate_row, v);
-          if (lane == 0) tma_store_wait_read<kOutBuffers - 1>();  // the buffer's last store has read it
+          if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
           __syncwarp();
-          uint8_t* b = out + buf * kOutBytes;
 #pragma unroll
           for (int q = 0; q < 4; ++q)  // 16-byte pieces in the 64-byte swizzle's places
             store_vec<T, kVec16<T>>(reinterpret_cast<T*>(b + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)),
@@ -393,7 +392,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (m0 < a.M && n < a.N) tma_store_2d(&tmY, n, m0, b);
             tma_store_commit();
           }
-          buf = buf + 1 == kOutBuffers ? 0 : buf + 1;
         } else if (row_ok) {
           // rows off 16 bytes, and the 16 columns that a tile of odd width leaves behind its last unit
           const int end = min(min(kU, sh.bn - c), a.N - n);
@@ -429,10 +427,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 template <typename T, bool kPair>
 void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
-  using Cfg = TileCfg<kPair>;
   constexpr int kCtas = kPair ? 2 : 1;
   auto kern = linear_tile_kernel<T, kPair>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   const CUtensorMap tmX = make_tmap_u8_2d(a.x, a.M, a.K, a.ldx, kBM);
   const CUtensorMap tmW = make_tmap_u8_2d(a.w, a.N, a.K, a.ldw, bn / kCtas);
   auto at = [](const void* p, int64_t bytes, int n) {
@@ -444,6 +441,8 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   sh.num_m = (a.M + kCtas * kBM - 1) / (kCtas * kBM);
   sh.num_n = (a.N + bn - 1) / bn;
   sh.num_k = (a.K + kBK - 1) / kBK;
+  sh.stage_bytes = (kBM + bn / kCtas) * kBK;
+  sh.stages = std::min(kMaxStages, (kSmemBytes - kSmemFixed) / sh.stage_bytes);
   sh.fast = at(a.y, a.ldy * e, 16) && at(a.residual, a.ldr * e, 16) && at(a.gate, a.gate_stride * 4, 16);
   const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
   const CUtensorMap tmY = sh.fast ? make_tmap_out_2d(a.y, type, sizeof(T), a.M, a.N, a.ldy, 32) : tmX;
@@ -453,7 +452,7 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kCtas * static_cast<unsigned>(tiles < slots ? tiles : slots));
   cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -465,14 +464,16 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, a, sh);
 }
 
-// Width of the tiles: the multiple of 16 whose rounds over the SMs cost least, a round being as long as
-// its tile is wide plus a fixed part (a narrow tile stages as many rows of x as a wide one).
+// Width of the tiles: the multiple of 16 whose rounds over the SMs cost least.  A k-block takes about 0.29 us +
+// 0.1 us * bn / 256 (8960 x 1536 channels at 32760 rows: 0.39, 0.355 and 0.325 us for 256, 192 and 128
+// channels), bound by the L2's traffic into shared memory more than by the products, so few wide rounds
+// beat many narrow ones, and a single round takes the narrowest tile that keeps it one.
 int pick_bn(int64_t num_m, int N, int slots) {
   int best = kMaxBn;
   int64_t cost = INT64_MAX;
   for (int bn = kMaxBn; bn >= 32; bn -= 16) {
     const int64_t tiles = num_m * ((N + bn - 1) / bn);
-    const int64_t c = (tiles + slots - 1) / slots * (bn + 48);
+    const int64_t c = (tiles + slots - 1) / slots * (bn + 740);
     if (c < cost) {
       cost = c;
       best = bn;
