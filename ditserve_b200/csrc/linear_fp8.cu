@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       fetch(tile + step);
       __syncwarp();
-      if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
+      if (!mbar_wait_warp(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kMaxBn;
 #pragma unroll 1

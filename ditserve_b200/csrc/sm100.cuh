@@ -106,6 +106,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same for a whole warp that goes on together: true for all lanes or for none, so that no lane leaves
+// alone and keeps the others waiting in the warp-wide instructions that follow.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                               int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
+}
+
 // ---------------------------------------------------------------------------
 // TMA (tensor copies global -> shared).  No multicast in any form.
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
@@ -117,6 +124,14 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
       "[%4];" ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -278,6 +293,11 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) |
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// The same with fp16 A and B (format 0).
+__host__ __device__ constexpr uint32_t umma_idesc_fp16(int M, int N, bool b_mn_major) {
+  return umma_idesc_bf16(M, N, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T on e4m3 inputs (K = 32 per instruction), fp32 accumulate; the

@@ -71,6 +71,22 @@ inline CUtensorMap make_tmap_u8_2d(const void* base, uint64_t rows, uint64_t col
   return map;
 }
 
+// [batch, rows, cols] of 2-byte elements in boxes of 1 x box_rows x 64 (one 128-byte swizzle atom wide);
+// strides in elements, multiples of 8.
+inline CUtensorMap make_tmap_16bit_3d(const void* base, uint64_t batch, uint64_t rows, uint64_t cols,
+                                      uint64_t row_stride, uint64_t batch_stride, uint32_t box_rows) {
+  CUtensorMap map;
+  cuuint64_t dims[3] = {cols, rows, batch};
+  cuuint64_t strides[2] = {row_stride * 2, batch_stride * 2};
+  cuuint32_t box[3] = {64, box_rows, 1};
+  cuuint32_t elem_strides[3] = {1, 1, 1};
+  CUresult r = encode_tiled_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box,
+                                 elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return map;
+}
+
 // A row-major output view of 2- or 4-byte elements in boxes of box_rows x 64 bytes (64-byte swizzle).
 inline CUtensorMap make_tmap_out_2d(void* base, CUtensorMapDataType type, int elem, uint64_t rows, uint64_t cols,
                                     uint64_t row_stride, uint32_t box_rows) {

@@ -49,7 +49,7 @@ def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _strided(t: torch.Tensor) -> torch.Tensor:
-    ok = t.stride(2) == 1 and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+    ok = t.stride(2) == 1 and t.stride(1) % 8 == 0 and (t.stride(1) > 0 or t.shape[1] == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
