@@ -1,265 +1,413 @@
 // torch bindings of the block operators: rms_norm_quant, linear_fp8, rope_axes, cross_attention.
-// As in bindings.cpp every rule that keeps a launch inside its buffers is checked here, so a bad call
-// raises a Python exception instead of reaching the GPU.
+//
+// Each entry checks its arguments, allocates what it returns and launches, in one call: at a few rows the
+// host's time is what a user waits for.  A call whose arguments are not laid out as its kernel takes them,
+// or are wrong, launches nothing and returns None; ops/ then either brings them into that layout and calls
+// again, or says what is wrong.  What keeps a launch inside its buffers is checked here alone.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
+#include <mutex>
 
 #include "kernels.h"
 
 namespace {
 
-int elem_type(const at::Tensor& t, const char* name) {
+namespace py = pybind11;
+using OptTensor = c10::optional<at::Tensor>;
+
+// The device status words that ops/_ext.py made, by device index.
+std::mutex status_mu;
+std::vector<at::Tensor> status_words;
+
+void bind_status(const at::Tensor& word) {
+  TORCH_CHECK(word.is_cuda() && word.scalar_type() == at::kInt && word.numel() >= 2 && word.is_contiguous(),
+              "a status word is int32 with 2 elements on a CUDA device");
+  std::lock_guard<std::mutex> lock(status_mu);
+  const size_t i = static_cast<size_t>(word.device().index());
+  if (status_words.size() <= i) status_words.resize(i + 1);
+  status_words[i] = word;
+}
+
+int* status_of(const at::Device& dev) {
+  std::lock_guard<std::mutex> lock(status_mu);
+  const size_t i = static_cast<size_t>(dev.index());
+  return i < status_words.size() && status_words[i].defined() ? status_words[i].data_ptr<int>() : nullptr;
+}
+
+int elem_type(const at::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return ds::kBF16;
     case at::kHalf: return ds::kFP16;
     case at::kFloat: return ds::kFP32;
-    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32");
+    default: return -1;
   }
 }
 
-void check_rows(const at::Tensor& t, const at::Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
-  TORCH_CHECK(t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1), name, " must be 2-D with unit column stride");
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
 }
 
-// an output's rows must not overlap each other
-void check_output(const at::Tensor& t, const at::Tensor& like, const char* name) {
-  check_rows(t, like, name);
-  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must have rows that do not overlap");
+// A tensor as rows of its last axis: any row stride in two dimensions, packed in more.
+struct Rows {
+  int64_t rows = 0, cols = 0, stride = 0;
+};
+
+bool as_rows(const at::Tensor& t, const at::Device& dev, Rows& r) {
+  const int64_t d = t.dim();
+  if (d < 1 || t.device() != dev) return false;
+  r.cols = t.size(d - 1);
+  if (r.cols <= 0 || r.cols >= (int64_t{1} << 30) || (r.cols > 1 && t.stride(d - 1) != 1)) return false;
+  if (d == 2) {
+    r.rows = t.size(0);
+    r.stride = t.stride(0);
+    return true;
+  }
+  r.rows = t.numel() / r.cols;
+  r.stride = r.cols;
+  return t.is_contiguous();
 }
 
-void check_vector(const at::Tensor& t, const at::Tensor& like, int64_t n, at::ScalarType type, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
-  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type, name, " must be ", type, " [", n, "]");
+// as_rows for a tensor that is written: its rows do not overlap each other
+bool as_output(const at::Tensor& t, const at::Device& dev, Rows& r) {
+  return as_rows(t, dev, r) && (r.rows <= 1 || r.stride >= r.cols);
 }
 
-void rms_norm_quant(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
-                    const c10::optional<at::Tensor>& residual, c10::optional<at::Tensor> h, at::Tensor& q,
-                    at::Tensor& scale, double eps) {
-  check_rows(x, x, "x");
+bool is_vector(const at::Tensor& t, const at::Device& dev, int64_t n, at::ScalarType type) {
+  return t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.device() == dev && (n <= 1 || t.stride(0) == 1);
+}
+
+// whether `out` (rows o) shares no byte with `in` (rows i): other storages, spans that do not meet, or other
+// columns of one buffer
+bool apart(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Rows& i) {
+  if (out.storage().data() != in.storage().data() || o.rows == 0 || i.rows == 0) return true;
+  const int64_t eo = out.element_size(), ei = in.element_size();
+  const int64_t lo = reinterpret_cast<int64_t>(out.data_ptr()), at = reinterpret_cast<int64_t>(in.data_ptr());
+  const int64_t hi = lo + ((o.rows - 1) * o.stride + o.cols) * eo, end = at + ((i.rows - 1) * i.stride + i.cols) * ei;
+  if (hi <= at || end <= lo) return true;
+  const int64_t pitch = i.stride * ei;
+  if (pitch <= 0 || o.stride * eo != pitch) return false;
+  const int64_t d = ((lo - at) % pitch + pitch) % pitch;
+  return d >= i.cols * ei && d + o.cols * eo <= pitch;
+}
+
+// ... or is `in` itself, element by element
+bool apart_or_same(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Rows& i) {
+  return apart(out, o, in, i) || (out.data_ptr() == in.data_ptr() && out.element_size() == in.element_size() &&
+                                  o.rows == i.rows && o.cols == i.cols && (o.rows <= 1 || o.stride == i.stride));
+}
+
+// whether the bytes that two tensors span meet
+bool spans_meet(const at::Tensor& x, const at::Tensor& y) {
+  auto span = [](const at::Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+    const int64_t lo = reinterpret_cast<int64_t>(t.data_ptr());
+    return std::make_pair(lo, lo + n * static_cast<int64_t>(t.element_size()));
+  };
+  const auto a = span(x), b = span(y);
+  return a.first < b.second && b.first < a.second;
+}
+
+// e4m3 of x's shape with rows that start on 16 bytes
+at::Tensor empty_fp8_like(const at::Tensor& x, const Rows& r) {
+  if (r.cols % 16 == 0) return empty(x.sizes(), at::kFloat8_e4m3fn, x.device());
+  const int64_t pitch = (r.cols + 15) / 16 * 16;
+  at::Tensor buf = empty({r.rows, pitch}, at::kFloat8_e4m3fn, x.device());
+  std::vector<int64_t> strides(x.dim(), 1);
+  int64_t s = pitch;
+  for (int64_t i = x.dim() - 2; i >= 0; --i) {
+    strides[i] = s;
+    s *= x.size(i);
+  }
+  return at::as_strided(buf, x.sizes(), strides);
+}
+
+py::object rms_norm_quant(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps,
+                          const OptTensor& out, const OptTensor& scale_out, const OptTensor& residual_out) {
+  const at::Device dev = x.device();
   ds::NormQuantArgs a;
-  a.type = elem_type(x, "x");
-  check_output(q, x, "out");
-  TORCH_CHECK(q.scalar_type() == at::kFloat8_e4m3fn && q.sizes() == x.sizes(), "out must be float8_e4m3fn of x's shape");
-  check_vector(scale, x, x.size(0), at::kFloat, "scale_out");
-  TORCH_CHECK(residual.has_value() == h.has_value(), "rms_norm_quant: a residual needs its output and the reverse");
-  if (residual.has_value()) {
-    check_rows(*residual, x, "residual");
-    check_output(*h, x, "residual_out");
-    TORCH_CHECK(residual->sizes() == x.sizes() && h->sizes() == x.sizes() &&
-                    residual->scalar_type() == x.scalar_type() && h->scalar_type() == x.scalar_type(),
-                "residual and residual_out must have x's shape and type");
-    a.residual = residual->data_ptr();
-    a.r_stride = residual->stride(0);
-    a.h = h->data_ptr();
-    a.h_stride = h->stride(0);
-  }
+  a.type = elem_type(x);
+  Rows rx, rr, rh, rq;
+  if (!x.is_cuda() || a.type < 0 || !as_rows(x, dev, rx)) return py::none();
   if (weight.has_value()) {
-    check_vector(*weight, x, x.size(1), x.scalar_type(), "weight");
-    TORCH_CHECK(weight->stride(0) == 1 || weight->size(0) == 1, "weight must be contiguous");
+    if (!is_vector(*weight, dev, rx.cols, x.scalar_type())) return py::none();
     a.weight = weight->data_ptr();
   }
-  TORCH_CHECK(x.size(1) > 0 && x.size(1) < (int64_t{1} << 30), "rms_norm_quant: bad row length");
-  const c10::cuda::CUDAGuard guard(x.device());
+  if (residual_out.has_value() && !residual.has_value()) return py::none();
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor h;
+  if (residual.has_value()) {
+    if (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type() || !as_rows(*residual, dev, rr))
+      return py::none();
+    if (residual_out.has_value()) {
+      h = *residual_out;
+      if (h.sizes() != x.sizes() || h.scalar_type() != x.scalar_type() || !as_output(h, dev, rh)) return py::none();
+      if (!apart_or_same(h, rh, x, rx) || !apart_or_same(h, rh, *residual, rr)) return py::none();
+    }
+  }
+  if (out.has_value() && (out->sizes() != x.sizes() || out->scalar_type() != at::kFloat8_e4m3fn || !as_output(*out, dev, rq)))
+    return py::none();
+  if (scale_out.has_value() && (scale_out->sizes() != x.sizes().slice(0, x.dim() - 1) || !scale_out->is_contiguous() ||
+                                scale_out->scalar_type() != at::kFloat || scale_out->device() != dev))
+    return py::none();
+  if (residual.has_value()) {
+    if (!residual_out.has_value()) {
+      h = empty(x.sizes(), x.scalar_type(), dev);
+      rh.stride = rx.cols;
+    }
+    a.residual = residual->data_ptr();
+    a.r_stride = rr.stride;
+    a.h = h.data_ptr();
+    a.h_stride = rh.stride;
+  }
+  at::Tensor q = out.has_value() ? *out : empty_fp8_like(x, rx);
+  if (!out.has_value()) rq.stride = (rx.cols + 15) / 16 * 16;
+  at::Tensor scale = scale_out.has_value() ? *scale_out : empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, dev);
   a.x = x.data_ptr();
-  a.x_stride = x.stride(0);
+  a.x_stride = rx.stride;
   a.q = reinterpret_cast<uint8_t*>(q.data_ptr());
-  a.q_stride = q.stride(0);
-  a.scale = scale.data_ptr<float>();
-  a.scale_stride = scale.stride(0);
-  a.rows = x.size(0);
-  a.dim = static_cast<int>(x.size(1));
+  a.q_stride = rq.stride;
+  a.scale = reinterpret_cast<float*>(scale.data_ptr());
+  a.rows = rx.rows;
+  a.dim = static_cast<int>(rx.cols);
   a.eps = static_cast<float>(eps);
   ds::launch_norm_quant(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return py::make_tuple(std::move(q), std::move(scale), residual.has_value() ? py::cast(std::move(h)) : py::none());
 }
 
-void linear_fp8(const at::Tensor& x, const at::Tensor& sx, const at::Tensor& w, const at::Tensor& sw, at::Tensor& y,
-                const c10::optional<at::Tensor>& bias, bool gelu, const c10::optional<at::Tensor>& residual,
-                const c10::optional<at::Tensor>& gate, int64_t rows_per_batch,
-                const c10::optional<at::Tensor>& row_batch, const at::Tensor& status) {
-  check_rows(x, x, "xq");
-  check_rows(w, x, "wq");
-  TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && w.scalar_type() == at::kFloat8_e4m3fn,
-              "xq and wq must be float8_e4m3fn");
-  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
-  TORCH_CHECK(w.size(1) == K, "linear_fp8: K mismatch");
-  TORCH_CHECK(K > 0 && K <= (1 << 30) && M <= (1 << 30) && N <= (1 << 30), "linear_fp8: sizes out of range");
-  for (const at::Tensor* t : {&x, &w})
-    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 &&
-                    (t->size(0) <= 1 || (t->stride(0) % 16 == 0 && t->stride(0) >= K)),
-                "xq and wq must have rows that start on 16 bytes");
-  check_vector(sx, x, M, at::kFloat, "x_scale");
-  check_vector(sw, x, N, at::kFloat, "w_scale");
-  check_output(y, x, "out");
-  TORCH_CHECK(y.size(0) == M && y.size(1) == N, "linear_fp8: out must be [", M, ", ", N, "]");
+// e4m3 rows that the product's 16-byte loads and tile loads can take
+bool fp8_rows(const at::Tensor& t, const at::Device& dev, Rows& r) {
+  if (t.scalar_type() != at::kFloat8_e4m3fn || !as_rows(t, dev, r)) return false;
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  if (r.rows <= 1) r.stride = (r.cols + 15) / 16 * 16;
+  return r.stride % 16 == 0 && r.stride >= r.cols;
+}
+
+py::object linear_fp8(const at::Tensor& x, const at::Tensor& sx, const at::Tensor& w, const at::Tensor& sw,
+                      const OptTensor& bias, bool gelu, const OptTensor& residual, const OptTensor& gate,
+                      c10::optional<int64_t> rows_per_batch, const OptTensor& row_batch, const OptTensor& out,
+                      at::ScalarType out_type) {
+  if (!x.is_cuda()) return py::none();
+  const at::Device dev = x.device();
+  Rows rx, rw, ry, rr;
   ds::LinearFp8Args a;
-  a.out_type = elem_type(y, "out");
+  a.status = status_of(dev);
+  if (a.status == nullptr || !fp8_rows(x, dev, rx) || w.dim() != 2 || !fp8_rows(w, dev, rw) || rw.cols != rx.cols)
+    return py::none();
+  const int64_t M = rx.rows, K = rx.cols, N = rw.rows;
+  if (M > (1 << 30) || N > (1 << 30)) return py::none();
+  if (sx.sizes() != x.sizes().slice(0, x.dim() - 1) || sx.scalar_type() != at::kFloat || sx.device() != dev ||
+      !sx.is_contiguous() || !is_vector(sw, dev, N, at::kFloat))
+    return py::none();
+  if (gelu && residual.has_value()) return py::none();
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  if (out.has_value()) {
+    out_type = out->scalar_type();
+    if (out->sizes() != at::IntArrayRef(shape) || (N > 0 && !as_output(*out, dev, ry))) return py::none();
+  } else {
+    ry.stride = N;
+  }
+  if (out_type != at::kBFloat16 && out_type != at::kHalf && out_type != at::kFloat) return py::none();
   if (bias.has_value()) {
-    check_vector(*bias, x, N, y.scalar_type(), "bias");
-    TORCH_CHECK(bias->stride(0) == 1 || N == 1, "bias must be contiguous");
+    if (!is_vector(*bias, dev, N, out_type)) return py::none();
     a.bias = bias->data_ptr();
   }
   if (residual.has_value()) {
-    check_rows(*residual, x, "residual");
-    TORCH_CHECK(residual->sizes() == y.sizes() && residual->scalar_type() == y.scalar_type(),
-                "residual must have out's shape and type");
+    if (residual->sizes() != at::IntArrayRef(shape) || residual->scalar_type() != out_type ||
+        (N > 0 && !as_rows(*residual, dev, rr)))
+      return py::none();
+    if (out.has_value() && N > 0 && !apart_or_same(*out, ry, *residual, rr)) return py::none();
     a.residual = residual->data_ptr();
-    a.ldr = residual->stride(0);
+    a.ldr = rr.stride;
   }
   if (gate.has_value()) {
-    check_rows(*gate, x, "gate");
-    TORCH_CHECK(residual.has_value(), "linear_fp8: a gate needs a residual");
-    TORCH_CHECK(gate->scalar_type() == at::kFloat && gate->size(1) == N && gate->size(0) >= 1, "gate must be fp32 [B, N]");
-    a.gate = gate->data_ptr<float>();
-    a.gate_stride = gate->stride(0);
-    a.batches = static_cast<int>(gate->size(0));
-    TORCH_CHECK(rows_per_batch > 0, "rows_per_batch must be positive");
-    a.rows_per_batch = static_cast<int>(std::min<int64_t>(rows_per_batch, 1 << 30));
+    const at::Tensor& g = *gate;
+    if (!residual.has_value() || g.scalar_type() != at::kFloat || g.device() != dev || g.dim() < 1 || g.dim() > 2 ||
+        g.size(-1) != N || (N > 1 && g.stride(-1) != 1))
+      return py::none();
+    const int64_t batches = g.dim() == 2 ? g.size(0) : 1;
+    const int64_t per = rows_per_batch.has_value() ? *rows_per_batch : std::max<int64_t>(M, 1);
+    if (batches < 1 || per < 1) return py::none();
+    a.gate = g.data_ptr<float>();
+    a.gate_stride = g.dim() == 2 ? g.stride(0) : 0;
+    a.batches = static_cast<int>(std::min<int64_t>(batches, 1 << 30));
+    a.rows_per_batch = static_cast<int>(std::min<int64_t>(per, 1 << 30));
     if (row_batch.has_value()) {
-      check_vector(*row_batch, x, M, at::kInt, "row_batch");
-      TORCH_CHECK(row_batch->stride(0) == 1 || M == 1, "row_batch must be contiguous");
+      if (!is_vector(*row_batch, dev, M, at::kInt)) return py::none();
       a.row_batch = row_batch->data_ptr<int>();
-    } else {
-      TORCH_CHECK((M + rows_per_batch - 1) / rows_per_batch <= gate->size(0), "gate has too few rows");
+    } else if ((M + per - 1) / per > batches) {
+      return py::none();
     }
   }
-  TORCH_CHECK(status.is_cuda() && status.device() == x.device() && status.scalar_type() == at::kInt && status.numel() >= 2,
-              "status must be int32 with 2 elements on ", x.device());
-  const c10::cuda::CUDAGuard guard(x.device());
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor y = out.has_value() ? *out : empty(shape, out_type, dev);
+  a.out_type = elem_type(y);
   a.x = reinterpret_cast<const uint8_t*>(x.data_ptr());
-  a.ldx = M > 1 ? x.stride(0) : (K + 15) / 16 * 16;
+  a.ldx = rx.stride;
   a.w = reinterpret_cast<const uint8_t*>(w.data_ptr());
-  a.ldw = N > 1 ? w.stride(0) : (K + 15) / 16 * 16;
-  a.sx = sx.data_ptr<float>();
-  a.sx_stride = sx.stride(0);
-  a.sw = sw.data_ptr<float>();
-  a.sw_stride = sw.stride(0);
+  a.ldw = rw.stride;
+  a.sx = reinterpret_cast<const float*>(sx.data_ptr());
+  a.sw = reinterpret_cast<const float*>(sw.data_ptr());
   a.y = y.data_ptr();
-  a.ldy = y.stride(0);
+  a.ldy = ry.stride;
   a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
   a.gelu = gelu ? 1 : 0;
-  a.status = status.data_ptr<int>();
   ds::launch_linear_fp8(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return py::cast(std::move(y));
 }
 
-void rope_axes(const at::Tensor& x, at::Tensor& y, const c10::optional<at::Tensor>& k, c10::optional<at::Tensor> ky,
-               const at::Tensor& pos, const std::vector<int64_t>& dims, const std::vector<double>& theta,
-               int64_t head_dim, bool half, bool inverse) {
+// What a rotation's axes and thetas fix: the axis and frequency of every pair.
+struct RopePlan {
+  int axes = 0, pairs = 0;
+  double turns[ds::kRopeMaxPairs];
+  uint8_t axis[ds::kRopeMaxPairs];
+};
+
+// None where the axes are not one to kRopeMaxAxes, each with positive even dims and a positive theta
+py::object rope_plan(const std::vector<int64_t>& dims, const std::vector<double>& theta) {
+  if (dims.empty() || dims.size() > ds::kRopeMaxAxes || dims.size() != theta.size()) return py::none();
+  int64_t pairs = 0;
+  for (size_t i = 0; i < dims.size(); ++i) {
+    if (dims[i] <= 0 || dims[i] % 2 != 0 || dims[i] > 2 * ds::kRopeMaxPairs || !(theta[i] > 0.0) || !std::isfinite(theta[i]))
+      return py::none();
+    pairs += dims[i] / 2;
+  }
+  if (pairs > ds::kRopeMaxPairs) return py::none();
+  RopePlan p;
+  p.axes = static_cast<int>(dims.size());
+  for (int i = 0; i < p.axes; ++i)
+    for (int64_t j = 0; j < dims[i] / 2; ++j, ++p.pairs) {
+      p.axis[p.pairs] = static_cast<uint8_t>(i);
+      p.turns[p.pairs] = std::pow(theta[i], -2.0 * static_cast<double>(j) / static_cast<double>(dims[i])) / (2.0 * M_PI);
+    }
+  return py::cast(p);
+}
+
+py::object rope_axes(const at::Tensor& x, const OptTensor& k, const at::Tensor& pos, const RopePlan& plan,
+                     int64_t head_dim, bool half, bool inverse, const OptTensor& out, const OptTensor& k_out) {
+  if (!x.is_cuda()) return py::none();
+  const at::Device dev = x.device();
   ds::RopeAxesArgs a;
-  a.type = elem_type(x, "x");
-  TORCH_CHECK(head_dim > 0 && head_dim <= (1 << 20), "rope_axes: bad head_dim");
-  const int64_t rows = x.size(0);
-  auto fill = [&](ds::RopeTensor& t, const at::Tensor& in, const at::Tensor& out, const char* name) {
-    check_rows(in, x, name);
-    check_output(out, x, "out");
-    TORCH_CHECK(in.scalar_type() == x.scalar_type() && out.scalar_type() == x.scalar_type() && in.size(0) == rows &&
-                    out.sizes() == in.sizes(),
-                "rope_axes: ", name, " and its output must agree in rows, shape and type");
-    TORCH_CHECK(in.size(1) % head_dim == 0 && in.size(1) < (int64_t{1} << 30), name, " must hold whole heads");
-    t.x = in.data_ptr();
-    t.x_stride = in.stride(0);
-    t.y = out.data_ptr();
-    t.y_stride = out.stride(0);
-    t.heads = static_cast<int>(in.size(1) / head_dim);
-  };
-  fill(a.t[0], x, y, "x");
-  TORCH_CHECK(k.has_value() == ky.has_value(), "rope_axes: k needs its output and the reverse");
-  if (k.has_value()) fill(a.t[1], *k, *ky, "k");
-  TORCH_CHECK(pos.is_cuda() && pos.device() == x.device() && pos.dim() == 2, "positions must be [P, axes] on ", x.device());
-  TORCH_CHECK(dims.size() >= 1 && dims.size() <= ds::kRopeMaxAxes && dims.size() == theta.size() &&
-                  pos.size(1) == static_cast<int64_t>(dims.size()),
-              "rope_axes: one to ", ds::kRopeMaxAxes, " axes, each with its dims, theta and position");
-  TORCH_CHECK(rows == 0 || (pos.size(0) > 0 && rows % pos.size(0) == 0), "rope_axes: rows must be a multiple of positions");
+  a.type = elem_type(x);
+  if (a.type < 0 || head_dim < 2 * plan.pairs || head_dim > (1 << 20) || (k_out.has_value() && !k.has_value()))
+    return py::none();
+  const int64_t pos_axes = pos.dim() == 1 ? 1 : (pos.dim() == 2 ? pos.size(1) : 0);
+  if (pos.device() != dev || pos_axes != plan.axes) return py::none();
   switch (pos.scalar_type()) {
     case at::kLong: a.pos_type = 0; break;
     case at::kInt: a.pos_type = 1; break;
     case at::kFloat: a.pos_type = 2; break;
     case at::kDouble: a.pos_type = 3; break;
-    default: TORCH_CHECK(false, "positions must be int64, int32, float32 or float64");
+    default: return py::none();
   }
-  int pairs = 0;
-  for (size_t i = 0; i < dims.size(); ++i) {
-    TORCH_CHECK(dims[i] > 0 && dims[i] % 2 == 0 && dims[i] <= head_dim && pairs + dims[i] / 2 <= ds::kRopeMaxPairs,
-                "rope_axes: dims must be positive, even, and at most ", 2 * ds::kRopeMaxPairs, " together");
-    for (int64_t j = 0; j < dims[i] / 2; ++j, ++pairs) {
-      a.axis[pairs] = static_cast<uint8_t>(i);
-      a.turns[pairs] = std::pow(theta[i], -2.0 * static_cast<double>(j) / static_cast<double>(dims[i])) / (2.0 * M_PI);
+  Rows in[2], to[2];
+  const at::Tensor* t[2] = {&x, k.has_value() ? &*k : nullptr};
+  const OptTensor* o[2] = {&out, &k_out};
+  for (int i = 0; i < 2 && t[i] != nullptr; ++i) {
+    if (t[i]->dim() < 2 || t[i]->scalar_type() != x.scalar_type() || !as_rows(*t[i], dev, in[i]) ||
+        in[i].cols % head_dim != 0 || in[i].rows != in[0].rows)
+      return py::none();
+    if (o[i]->has_value()) {
+      const at::Tensor& y = **o[i];
+      if (y.sizes() != t[i]->sizes() || y.scalar_type() != x.scalar_type() || !as_output(y, dev, to[i]) ||
+          !apart_or_same(y, to[i], *t[i], in[i]))
+        return py::none();
+    } else {
+      to[i].stride = in[i].cols;
     }
   }
-  TORCH_CHECK(2 * pairs <= head_dim, "rope_axes: dims exceed head_dim");
-  const c10::cuda::CUDAGuard guard(x.device());
+  // with k: neither output on the other's input, nor the outputs on each other
+  if (k.has_value() && ((out.has_value() && !apart(*out, to[0], *k, in[1])) ||
+                        (k_out.has_value() && !apart(*k_out, to[1], x, in[0])) ||
+                        (out.has_value() && k_out.has_value() && !apart(*out, to[0], *k_out, to[1]))))
+    return py::none();
+  const int64_t rows = in[0].rows;
+  if (rows > 0 && (pos.size(0) == 0 || rows % pos.size(0) != 0)) return py::none();
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor y[2];
+  for (int i = 0; i < 2 && t[i] != nullptr; ++i) {
+    y[i] = o[i]->has_value() ? **o[i] : empty(t[i]->sizes(), x.scalar_type(), dev);
+    a.t[i].x = t[i]->data_ptr();
+    a.t[i].x_stride = in[i].stride;
+    a.t[i].y = y[i].data_ptr();
+    a.t[i].y_stride = to[i].stride;
+    a.t[i].heads = static_cast<int>(in[i].cols / head_dim);
+  }
   a.rows = rows;
   a.head_dim = static_cast<int>(head_dim);
-  a.pairs = pairs;
+  a.pairs = plan.pairs;
   a.half = half ? 1 : 0;
   a.inverse = inverse ? 1 : 0;
   a.pos = pos.data_ptr();
   a.pos_rows = pos.size(0);
   a.pos_stride = pos.stride(0);
-  a.axis_stride = pos.stride(1);
+  a.axis_stride = pos.dim() == 2 ? pos.stride(1) : 0;
+  std::copy(plan.turns, plan.turns + plan.pairs, a.turns);
+  std::copy(plan.axis, plan.axis + plan.pairs, a.axis);
   ds::launch_rope_axes(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (t[1] == nullptr) return py::cast(std::move(y[0]));
+  return py::make_tuple(std::move(y[0]), std::move(y[1]));
 }
 
-void cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
-                     c10::optional<at::Tensor> lse, const c10::optional<at::Tensor>& kv_lens,
-                     const c10::optional<at::Tensor>& key_mask, int64_t heads, int64_t heads_kv, int64_t head_dim,
-                     double scale, const at::Tensor& status) {
+py::object cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t heads, int64_t heads_kv,
+                           const OptTensor& kv_lens, const OptTensor& key_mask, c10::optional<double> scale,
+                           const OptTensor& out, bool return_lse) {
+  if (!q.is_cuda() || q.dim() != 3 || k.dim() != 3 || heads < 1 || heads_kv < 1 || heads % heads_kv != 0) return py::none();
+  const at::Device dev = q.device();
   ds::CrossAttnArgs a;
-  a.type = elem_type(q, "q");
-  TORCH_CHECK(q.is_cuda() && q.dim() == 3, "q must be a CUDA tensor [B, Sq, heads * head_dim]");
-  const int64_t B = q.size(0), Sq = q.size(1), Sk = k.dim() == 3 ? k.size(1) : -1;
-  TORCH_CHECK(heads > 0 && heads_kv > 0 && heads % heads_kv == 0, "cross_attention: heads must be a multiple of heads_kv");
-  TORCH_CHECK(B <= 65535 && heads_kv <= 65535 && Sk > 0 && Sk < (int64_t{1} << 30) &&
-                  Sq * (heads / heads_kv) < (int64_t{1} << 30) && heads * head_dim < (int64_t{1} << 30),
-              "cross_attention: sizes out of range");
-  auto check = [&](const at::Tensor& t, int64_t rows, int64_t width, const char* name, bool output) {
-    TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.scalar_type() == q.scalar_type(), name,
-                " must have q's device and type");
-    TORCH_CHECK(t.dim() == 3 && t.size(0) == B && t.size(1) == rows && t.size(2) == width, name, " must be [", B, ", ",
-                rows, ", ", width, "]");
-    TORCH_CHECK(t.stride(2) == 1 && t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 &&
-                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-                name, " must have rows that start on 16 bytes");
-    if (output)
-      TORCH_CHECK((rows <= 1 || t.stride(1) >= width) && (B <= 1 || t.stride(0) >= width), name,
-                  " must have rows that do not overlap");
+  a.type = elem_type(q);
+  a.status = status_of(dev);
+  const int64_t B = q.size(0), Sq = q.size(1), width = q.size(2), Sk = k.size(1), d = width / heads;
+  if (a.status == nullptr || (a.type != ds::kBF16 && a.type != ds::kFP16) || width % heads != 0 || (d != 64 && d != 128))
+    return py::none();
+  if (B < 1 || B > 65535 || heads_kv > 65535 || Sq < 1 || Sk < 1 || Sk >= (int64_t{1} << 30) ||
+      Sq * (heads / heads_kv) >= (int64_t{1} << 30) || width >= (int64_t{1} << 30))
+    return py::none();
+  auto fits = [&](const at::Tensor& t, int64_t rows, int64_t cols, bool output) {
+    if (t.device() != dev || t.scalar_type() != q.scalar_type() || t.dim() != 3 || t.size(0) != B || t.size(1) != rows ||
+        t.size(2) != cols || t.stride(2) != 1 || t.stride(1) % 8 != 0 || t.stride(0) % 8 != 0 ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
+      return false;
+    if (rows > 1 && t.stride(1) < (output ? cols : 8)) return false;
+    return !output || B == 1 || t.stride(0) >= cols;
   };
-  check(q, Sq, heads * head_dim, "q", false);
-  check(k, Sk, heads_kv * head_dim, "k", false);
-  check(v, Sk, heads_kv * head_dim, "v", false);
-  check(o, Sq, heads * head_dim, "out", true);
-  if (lse.has_value()) {
-    TORCH_CHECK(lse->is_cuda() && lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() &&
-                    lse->numel() == B * heads * Sq,
-                "lse must be contiguous fp32 [B, heads, Sq]");
-    a.lse = lse->data_ptr<float>();
+  if (!fits(q, Sq, width, false) || !fits(k, Sk, heads_kv * d, false) || !fits(v, Sk, heads_kv * d, false)) return py::none();
+  if (out.has_value()) {
+    if (!fits(*out, Sq, width, true)) return py::none();
+    for (const at::Tensor* t : {&q, &k, &v})
+      if (spans_meet(*out, *t)) return py::none();
   }
-  at::Tensor lens;
   if (kv_lens.has_value()) {
-    check_vector(*kv_lens, q, B, at::kInt, "kv_lens");
-    lens = kv_lens->contiguous();
-    a.kv_lens = lens.data_ptr<int>();
+    if (!is_vector(*kv_lens, dev, B, at::kInt)) return py::none();
+    a.kv_lens = kv_lens->data_ptr<int>();
   }
   if (key_mask.has_value()) {
-    TORCH_CHECK(key_mask->is_cuda() && key_mask->device() == q.device() && key_mask->scalar_type() == at::kBool &&
-                    key_mask->dim() == 2 && key_mask->size(0) == B && key_mask->size(1) == Sk,
-                "key_mask must be bool [", B, ", ", Sk, "]");
-    a.key_mask = reinterpret_cast<const uint8_t*>(key_mask->data_ptr());
-    a.mask_row = key_mask->stride(0);
-    a.mask_col = key_mask->stride(1);
+    const at::Tensor& m = *key_mask;
+    if (m.device() != dev || m.scalar_type() != at::kBool || m.dim() != 2 || m.size(0) != B || m.size(1) != Sk)
+      return py::none();
+    a.key_mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
+    a.mask_row = m.stride(0);
+    a.mask_col = m.stride(1);
   }
-  TORCH_CHECK(status.is_cuda() && status.device() == q.device() && status.scalar_type() == at::kInt && status.numel() >= 2,
-              "status must be int32 with 2 elements on ", q.device());
-  const c10::cuda::CUDAGuard guard(q.device());
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(d));
+  if (!(s > 0.0) || !std::isfinite(s)) return py::none();
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor o = out.has_value() ? *out : empty(q.sizes(), q.scalar_type(), dev), lse;
+  if (return_lse) {
+    lse = empty({B, heads, Sq}, at::kFloat, dev);
+    a.lse = lse.data_ptr<float>();
+  }
   a.q = q.data_ptr();
   a.k = k.data_ptr();
   a.v = v.data_ptr();
@@ -273,18 +421,22 @@ void cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   a.seq_k = static_cast<int>(Sk);
   a.heads = static_cast<int>(heads);
   a.heads_kv = static_cast<int>(heads_kv);
-  a.head_dim = static_cast<int>(head_dim);
-  a.scale = static_cast<float>(scale);
-  a.status = status.data_ptr<int>();
+  a.head_dim = static_cast<int>(d);
+  a.scale = static_cast<float>(s);
   ds::launch_cross_attention(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (!return_lse) return py::cast(std::move(o));
+  return py::make_tuple(std::move(o), std::move(lse));
 }
 
 }  // namespace
 
 void bind_block_ops(pybind11::module_& m) {
+  m.def("bind_status", &bind_status, "names a device's status word to the block operators");
   m.def("rms_norm_quant", &rms_norm_quant, "residual addition + RMS norm + e4m3 rows with scales");
   m.def("linear_fp8", &linear_fp8, "linear layer on e4m3 operands with row scales");
+  py::class_<RopePlan>(m, "RopePlan");
+  m.def("rope_plan", &rope_plan, "the frequencies of a set of axes, or None");
   m.def("rope_axes", &rope_axes, "rotary positions with several axes");
   m.def("cross_attention", &cross_attention, "attention to padded, masked encoder states");
 }

@@ -250,21 +250,24 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Many queries: persistent CTAs on the tensor cores (tcgen05).  A unit of work is up to 256 queries of one head
-// in two 128-row tiles A and B, against all key tiles of its batch entry.
+// Many queries: persistent CTAs on the tensor cores (tcgen05).  A unit of work is two 128-row tiles A and B of
+// the query rows that read one key head (its heads' tiles in turn), against all key tiles of the batch entry.
 //   warp 0        TMA: Q of both tiles, K one tile ahead of V
 //   warp 1        products, in the order S_A(i+1) after PV_A(i), S_B(i+1) after PV_B(i), straight on over the
-//                 end of a unit: the next unit's first scores are formed while this one's last softmax and
-//                 its output run
+//                 end of a unit
 //   warp 2        puts zeros in the values of masked keys (only with lengths or a mask)
-//   warps 4..7    softmax and output of tile A, a row a thread; warps 8..11 of tile B
+//   warps 4..7    softmax of tile A, a row a thread; warps 8..11 of tile B
+//   warps 12..15  outputs: O / l from TMEM to memory, while the softmax goes on with the next unit
 // TMEM: S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B [384, 384 + D).  P is written over the first
 // half of its S as the second product's TMEM operand.  O is rescaled only when the running maximum has grown by
 // more than 2^8, P then is at most 256 and exact sums hold in fp32.
 // An encoder's context is a few key tiles long, so a unit is short: what makes the kernel fast is
 // that nothing drains between units.  Bound by the exponentials and the products about equally.
 constexpr int kQT = 128, kKT = 128, kPChunks = 2;
-constexpr int kTileThreads = 384;
+constexpr int kTileThreads = 512;
+// registers a thread: 512 threads start with 128; loaders and output warps give to the softmax warps
+constexpr int kRegsOther = 88, kRegsSoftmax = 168;
+static_assert(2 * kRegsOther + 2 * kRegsSoftmax <= 4 * 128, "more registers than the block starts with");
 
 template <int D>
 struct TileCfg {
@@ -272,7 +275,7 @@ struct TileCfg {
   static constexpr int kQBytes = kQT * D * 2;
   static constexpr int kKvBytes = kKT * D * 2;
   static constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
-  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 1024 + 512;
+  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 2 * kQT * 8 + 1024 + 512;
 };
 
 struct TileMaps {
@@ -280,7 +283,7 @@ struct TileMaps {
 };
 
 struct TileShape {
-  int units, q_blocks;  // unit = (b * heads + h) * q_blocks + query block of 256
+  int units, pairs, q_tiles;         // unit = (b * heads_kv + hk) * pairs + pair of row tiles
   int k_shared, v_shared, q_shared;  // batch stride 0: one entry read by all
   int wide_out;                      // rows of o start on 32 bytes
 };
@@ -299,20 +302,31 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 struct Unit {
-  int b, h, q0, n;  // batch entry, head, first query, key tiles
-  bool two;         // tile B has queries
+  int b, hk, pair, n;  // batch entry, key head, pair of row tiles, key tiles
+  bool two;            // tile B has rows
 };
 
 __device__ __forceinline__ Unit unit_of(const CrossAttnArgs& a, const TileShape& sh, int u) {
   Unit x;
-  const int bh = u / sh.q_blocks;
-  x.b = bh / a.heads;
-  x.h = bh - x.b * a.heads;
-  x.q0 = (u - bh * sh.q_blocks) * 2 * kQT;
+  const int bh = u / sh.pairs;
+  x.pair = u - bh * sh.pairs;
+  x.b = bh / a.heads_kv;
+  x.hk = bh - x.b * a.heads_kv;
   x.n = (valid_keys(a, x.b) + kKT - 1) / kKT;
-  x.two = a.seq_q - x.q0 > kQT;
+  x.two = 2 * x.pair + 1 < sh.q_tiles * (a.heads / a.heads_kv);
   return x;
 }
+
+// head and first query of tile t of a unit
+__device__ __forceinline__ int2 tile_of(const CrossAttnArgs& a, const TileShape& sh, const Unit& x, int t) {
+  const int i = 2 * x.pair + t, g = i / sh.q_tiles;
+  return make_int2(x.hk * (a.heads / a.heads_kv) + g, (i - g * sh.q_tiles) * kQT);
+}
+
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
 // One key tile of one unit; walks a CTA's units in order, leaving out those without keys.
 struct Step {
@@ -351,7 +365,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * Cfg::kQBytes;
   uint8_t* sV = sK + ST * Cfg::kKvBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kKvBytes);  // [2] a tile
+  float2* row_ml = reinterpret_cast<float2*>(sV + ST * Cfg::kKvBytes);  // [2][128] maximum and sum of a finished row
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(row_ml + 2 * kQT);     // [2] a tile
   uint64_t* q_empty = q_full + 2;
   uint64_t* k_full = q_empty + 2;   // [ST]
   uint64_t* k_empty = k_full + ST;
@@ -361,7 +376,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* s_full = v_empty + ST;           // [2]
   uint64_t* p_full = s_full + 2;             // [2][kPChunks]
   uint64_t* pv_done = p_full + 2 * kPChunks;  // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint64_t* l_full = pv_done + 2;   // [2] row_ml written
+  uint64_t* o_empty = l_full + 2;   // [2] O and row_ml read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,6 +390,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&l_full[i], 128);
+      mbar_init(&o_empty[i], 128);
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
@@ -391,159 +410,167 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- TMA ----------------
-      tma_prefetch_desc(&maps.q);
-      tma_prefetch_desc(&maps.k);
-      tma_prefetch_desc(&maps.v);
-      const int group = a.heads / a.heads_kv;
-      int q_count[2] = {0, 0}, kc = 0, vc = 0;
-      auto load_q = [&](const Unit& x) -> bool {
-        for (int t = 0; t < (x.two ? 2 : 1); ++t) {
-          if (!mbar_wait(&q_empty[t], (q_count[t] & 1) ^ 1, abort_flag, a.status, 410 + t)) return false;
-          ++q_count[t];
-          mbar_arrive_expect_tx(&q_full[t], Cfg::kQBytes);
-#pragma unroll
-          for (int i = 0; i < Cfg::kAtoms; ++i)
-            tma_load_3d(sQ + t * Cfg::kQBytes + i * (kQT * 128), &maps.q, x.h * D + i * 64, x.q0 + t * kQT,
-                        sh.q_shared ? 0 : x.b, &q_full[t]);
-        }
-        return true;
-      };
-      auto load_kv = [&](const Step& s, const CUtensorMap* map, int shared, uint8_t* base, uint64_t* full, uint64_t* empty,
-                         int& count, int site) -> bool {
-        const int st = count % ST;
-        if (!mbar_wait(&empty[st], ((count / ST) & 1) ^ 1, abort_flag, a.status, site)) return false;
-        ++count;
-        mbar_arrive_expect_tx(&full[st], Cfg::kKvBytes);
-#pragma unroll
-        for (int i = 0; i < Cfg::kAtoms; ++i)
-          tma_load_3d(base + st * Cfg::kKvBytes + i * (kKT * 128), map, (s.x.h / group) * D + i * 64, s.j * kKT,
-                      shared ? 0 : s.x.b, &full[st]);
-        return true;
-      };
-      Step cur;
-      cur.u = blockIdx.x;
-      bool ok = cur.settle(a, sh) && load_q(cur.x) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412);
-      while (ok) {
-        Step next = cur;
-        const bool more = next.advance(a, sh);
-        if (more) {
-          if (next.j == 0 && !load_q(next.x)) break;
-          if (!load_kv(next, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412)) break;
-        }
-        if (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
-        cur = next;
-        ok = more;
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- products ----------------
-      constexpr uint32_t idesc_s = kBf16 ? umma_idesc_bf16(kQT, kKT, false) : umma_idesc_fp16(kQT, kKT, false);
-      constexpr uint32_t idesc_o = kBf16 ? umma_idesc_bf16(kQT, D, true) : umma_idesc_fp16(kQT, D, true);
-      int q_count[2] = {0, 0}, p_count[2] = {0, 0}, kc = 0, vc = 0;
-      uint64_t* v_go = masked_kv ? v_ready : v_full;
-      // S_t = Q_t K^T of step s, whose K is the kc-th
-      auto issue_s = [&](int t, const Step& s) -> bool {
-        if (s.j == 0) {
-          if (!mbar_wait(&q_full[t], q_count[t] & 1, abort_flag, a.status, 420 + t)) return false;
-          ++q_count[t];
-        }
-        const int st = kc % ST;
-        if (t == 0) {
-          if (!mbar_wait(&k_full[st], (kc / ST) & 1, abort_flag, a.status, 422)) return false;
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kQT * 128) + (kk & 3) * 32;
-          const uint64_t da = umma_desc_sw128(smem_u32(sQ + t * Cfg::kQBytes) + off, 16, 1024);
-          const uint64_t db = umma_desc_sw128(smem_u32(sK + st * Cfg::kKvBytes) + off, 16, 1024);
-          umma_bf16_ss(tmem_base + t * kKT, da, db, idesc_s, kk != 0);
-        }
-        umma_commit(&s_full[t]);
-        if (s.j + 1 == s.x.n) umma_commit(&q_empty[t]);
-        return true;
-      };
-      // O_t (+)= P_t V of step s, whose V is the vc-th
-      auto issue_pv = [&](int t, const Step& s) -> bool {
-        const uint32_t v_base = smem_u32(sV + (vc % ST) * Cfg::kKvBytes);
-        constexpr int kPer = kKT / 16 / kPChunks;
-#pragma unroll
-        for (int c = 0; c < kPChunks; ++c) {
-          if (!mbar_wait(&p_full[t * kPChunks + c], p_count[t] & 1, abort_flag, a.status, 424 + t)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int kk = c * kPer + i;
-            const uint64_t db = umma_desc_sw128(v_base + kk * (16 * 128), kKT * 128, 1024);
-            umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * kKT + kk * 8, db, idesc_o, (s.j | kk) != 0);
+  if (warp < 4) {
+    regs_dec<kRegsOther>();
+    if (warp == 0) {
+      if (lane == 0) {
+        // ---------------- TMA ----------------
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+        int q_count[2] = {0, 0}, kc = 0, vc = 0;
+        auto load_q = [&](const Unit& x) -> bool {
+          for (int t = 0; t < (x.two ? 2 : 1); ++t) {
+            if (!mbar_wait(&q_empty[t], (q_count[t] & 1) ^ 1, abort_flag, a.status, 410 + t)) return false;
+            ++q_count[t];
+            mbar_arrive_expect_tx(&q_full[t], Cfg::kQBytes);
+            const int2 at = tile_of(a, sh, x, t);
+  #pragma unroll
+            for (int i = 0; i < Cfg::kAtoms; ++i)
+              tma_load_3d(sQ + t * Cfg::kQBytes + i * (kQT * 128), &maps.q, at.x * D + i * 64, at.y,
+                          sh.q_shared ? 0 : x.b, &q_full[t]);
           }
+          return true;
+        };
+        auto load_kv = [&](const Step& s, const CUtensorMap* map, int shared, uint8_t* base, uint64_t* full, uint64_t* empty,
+                           int& count, int site) -> bool {
+          const int st = count % ST;
+          if (!mbar_wait(&empty[st], ((count / ST) & 1) ^ 1, abort_flag, a.status, site)) return false;
+          ++count;
+          mbar_arrive_expect_tx(&full[st], Cfg::kKvBytes);
+  #pragma unroll
+          for (int i = 0; i < Cfg::kAtoms; ++i)
+            tma_load_3d(base + st * Cfg::kKvBytes + i * (kKT * 128), map, s.x.hk * D + i * 64, s.j * kKT,
+                        shared ? 0 : s.x.b, &full[st]);
+          return true;
+        };
+        Step cur;
+        cur.u = blockIdx.x;
+        bool ok = cur.settle(a, sh) && load_q(cur.x) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412);
+        while (ok) {
+          Step next = cur;
+          const bool more = next.advance(a, sh);
+          if (more) {
+            if (next.j == 0 && !load_q(next.x)) break;
+            if (!load_kv(next, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412)) break;
+          }
+          if (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
+          cur = next;
+          ok = more;
         }
-        ++p_count[t];
-        umma_commit(&pv_done[t]);
-        return true;
-      };
-      Step cur;
-      cur.u = blockIdx.x;
-      bool ok = cur.settle(a, sh);
-      if (ok) {
-        ok = issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
-        umma_commit(&k_empty[kc % ST]);
-        ++kc;
       }
-      while (ok) {
-        Step next = cur;
-        const bool more = next.advance(a, sh);
-        if (!mbar_wait(&v_go[vc % ST], (vc / ST) & 1, abort_flag, a.status, 423)) break;
-        tc_fence_after();
-        if (!issue_pv(0, cur)) break;
-        if (more && !issue_s(0, next)) break;
-        if (cur.x.two && !issue_pv(1, cur)) break;
-        umma_commit(&v_empty[vc % ST]);
-        ++vc;
-        if (more) {
-          if (next.x.two && !issue_s(1, next)) break;
+    } else if (warp == 1) {
+      if (lane == 0) {
+        // ---------------- products ----------------
+        constexpr uint32_t idesc_s = kBf16 ? umma_idesc_bf16(kQT, kKT, false) : umma_idesc_fp16(kQT, kKT, false);
+        constexpr uint32_t idesc_o = kBf16 ? umma_idesc_bf16(kQT, D, true) : umma_idesc_fp16(kQT, D, true);
+        int q_count[2] = {0, 0}, p_count[2] = {0, 0}, o_count[2] = {0, 0}, kc = 0, vc = 0;
+        uint64_t* v_go = masked_kv ? v_ready : v_full;
+        // S_t = Q_t K^T of step s, whose K is the kc-th
+        auto issue_s = [&](int t, const Step& s) -> bool {
+          if (s.j == 0) {
+            if (!mbar_wait(&q_full[t], q_count[t] & 1, abort_flag, a.status, 420 + t)) return false;
+            ++q_count[t];
+          }
+          const int st = kc % ST;
+          if (t == 0) {
+            if (!mbar_wait(&k_full[st], (kc / ST) & 1, abort_flag, a.status, 422)) return false;
+          }
+          tc_fence_after();
+  #pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kQT * 128) + (kk & 3) * 32;
+            const uint64_t da = umma_desc_sw128(smem_u32(sQ + t * Cfg::kQBytes) + off, 16, 1024);
+            const uint64_t db = umma_desc_sw128(smem_u32(sK + st * Cfg::kKvBytes) + off, 16, 1024);
+            umma_bf16_ss(tmem_base + t * kKT, da, db, idesc_s, kk != 0);
+          }
+          umma_commit(&s_full[t]);
+          if (s.j + 1 == s.x.n) umma_commit(&q_empty[t]);
+          return true;
+        };
+        // O_t (+)= P_t V of step s, whose V is the vc-th
+        auto issue_pv = [&](int t, const Step& s) -> bool {
+          const uint32_t v_base = smem_u32(sV + (vc % ST) * Cfg::kKvBytes);
+          constexpr int kPer = kKT / 16 / kPChunks;
+          if (s.j == 0) {  // the unit before has been written out
+            if (!mbar_wait(&o_empty[t], (o_count[t] & 1) ^ 1, abort_flag, a.status, 426 + t)) return false;
+            ++o_count[t];
+          }
+  #pragma unroll
+          for (int c = 0; c < kPChunks; ++c) {
+            if (!mbar_wait(&p_full[t * kPChunks + c], p_count[t] & 1, abort_flag, a.status, 424 + t)) return false;
+            tc_fence_after();
+  #pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const int kk = c * kPer + i;
+              const uint64_t db = umma_desc_sw128(v_base + kk * (16 * 128), kKT * 128, 1024);
+              umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * kKT + kk * 8, db, idesc_o, (s.j | kk) != 0);
+            }
+          }
+          ++p_count[t];
+          umma_commit(&pv_done[t]);
+          return true;
+        };
+        Step cur;
+        cur.u = blockIdx.x;
+        bool ok = cur.settle(a, sh);
+        if (ok) {
+          ok = issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
           umma_commit(&k_empty[kc % ST]);
           ++kc;
         }
-        cur = next;
-        ok = more;
+        while (ok) {
+          Step next = cur;
+          const bool more = next.advance(a, sh);
+          if (!mbar_wait(&v_go[vc % ST], (vc / ST) & 1, abort_flag, a.status, 423)) break;
+          tc_fence_after();
+          if (!issue_pv(0, cur)) break;
+          if (more && !issue_s(0, next)) break;
+          if (cur.x.two && !issue_pv(1, cur)) break;
+          umma_commit(&v_empty[vc % ST]);
+          ++vc;
+          if (more) {
+            if (next.x.two && !issue_s(1, next)) break;
+            umma_commit(&k_empty[kc % ST]);
+            ++kc;
+          }
+          cur = next;
+          ok = more;
+        }
       }
-    }
-  } else if (warp == 2) {
-    if (masked_kv) {
-      // ---------------- values of masked keys ----------------
-      Step s;
-      s.u = blockIdx.x;
-      int vc = 0;
-      for (bool ok = s.settle(a, sh); ok; ok = s.advance(a, sh), ++vc) {
-        const int st = vc % ST;
-        uint32_t w[4];
-        tile_mask(a, s.x.b, s.j, valid_keys(a, s.x.b), w);
-        // every lane waits, so that what TMA wrote is ordered before its stores
-        if (!mbar_wait_warp(&v_full[st], (vc / ST) & 1, abort_flag, a.status, 430)) break;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!((w[i] >> lane) & 1)) {
-#pragma unroll
-            for (int c = 0; c < Cfg::kAtoms; ++c) {
-              // a key's 64 values are one 128-byte row of the atom, however its pieces are swizzled
-              uint4* row = reinterpret_cast<uint4*>(sV + st * Cfg::kKvBytes + c * (kKT * 128) + (i * 32 + lane) * 128);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) row[(e + lane) & 7] = make_uint4(0, 0, 0, 0);
+    } else if (warp == 2) {
+      if (masked_kv) {
+        // ---------------- values of masked keys ----------------
+        Step s;
+        s.u = blockIdx.x;
+        int vc = 0;
+        for (bool ok = s.settle(a, sh); ok; ok = s.advance(a, sh), ++vc) {
+          const int st = vc % ST;
+          uint32_t w[4];
+          tile_mask(a, s.x.b, s.j, valid_keys(a, s.x.b), w);
+          // every lane waits, so that what TMA wrote is ordered before its stores
+          if (!mbar_wait_warp(&v_full[st], (vc / ST) & 1, abort_flag, a.status, 430)) break;
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!((w[i] >> lane) & 1)) {
+  #pragma unroll
+              for (int c = 0; c < Cfg::kAtoms; ++c) {
+                // a key's 64 values are one 128-byte row of the atom, however its pieces are swizzled
+                uint4* row = reinterpret_cast<uint4*>(sV + st * Cfg::kKvBytes + c * (kKT * 128) + (i * 32 + lane) * 128);
+  #pragma unroll
+                for (int e = 0; e < 8; ++e) row[(e + lane) & 7] = make_uint4(0, 0, 0, 0);
+              }
             }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ready[st]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_ready[st]);
       }
     }
-  } else if (warp >= 4) {
-    // ---------------- softmax and output of tile t ----------------
+  } else if (warp < 12) {
+    regs_inc<kRegsSoftmax>();
+    // ---------------- softmax of tile t ----------------
     const int t = (warp >> 2) - 1;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -553,10 +580,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const float sl2 = a.scale * kLog2e;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     int step = 0;  // key tiles of tile t so far: the phase of its barriers
+    int done = 0;  // units of tile t so far
     bool ok = true;
     for (int u = blockIdx.x; ok && u < sh.units; u += gridDim.x) {
       const Unit x = unit_of(a, sh, u);
-      if (t == 1 && !x.two) continue;
+      if (x.n == 0 || (t == 1 && !x.two)) continue;
       const int valid = valid_keys(a, x.b);
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < x.n; ++j, ++step) {
@@ -659,47 +687,81 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       if (!ok) break;
-      const int i_q = x.q0 + t * kQT + row;
-      const bool row_ok = i_q < a.seq_q;
-      T* out = reinterpret_cast<T*>(a.o) + x.b * a.o_batch + static_cast<int64_t>(i_q) * a.o_row + x.h * D;
-      if (x.n > 0) {
-        if (!mbar_wait_warp(&pv_done[t], (step - 1) & 1, abort_flag, a.status, 444 + t)) break;
-        tc_fence_after();
-      }
-      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // no key: the sums of O are zero too
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
+      // the output warps have read the unit before
+      if (!mbar_wait_warp(&o_empty[t], (done & 1) ^ 1, abort_flag, a.status, 444 + t)) break;
+      ++done;
+      row_ml[t * kQT + row] = make_float2(m_run, l_run);
+      mbar_arrive(&l_full[t]);
+    }
+  } else {
+    regs_dec<kRegsOther>();
+    // ---------------- outputs ----------------
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    int step[2] = {0, 0}, done[2] = {0, 0};
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < sh.units; u += gridDim.x) {
+      const Unit x = unit_of(a, sh, u);
+      for (int t = 0; t < (x.two ? 2 : 1); ++t) {
+        const int2 at = tile_of(a, sh, x, t);
+        const int i_q = at.y + row;
+        const bool row_ok = i_q < a.seq_q;
+        T* out = reinterpret_cast<T*>(a.o) + x.b * a.o_batch + static_cast<int64_t>(i_q) * a.o_row + at.x * D;
+        float m = -INFINITY, l = 0.f;
         if (x.n > 0) {
-          tmem_ld32(o_col + c * 32, o);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
+          if (!mbar_wait_warp(&l_full[t], done[t] & 1, abort_flag, a.status, 450 + t)) {
+            ok = false;
+            break;
+          }
+          ++done[t];
+          const float2 ml = row_ml[t * kQT + row];
+          m = ml.x;
+          l = ml.y;
+          step[t] += x.n;
+          if (!mbar_wait_warp(&pv_done[t], (step[t] - 1) & 1, abort_flag, a.status, 452 + t)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
         }
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          p[e] = pack2(T(), __uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-        if (row_ok) {
-          if (sh.wide_out) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c * 32 + h * 16),
-                           "r"(p[8 * h]), "r"(p[8 * h + 1]), "r"(p[8 * h + 2]), "r"(p[8 * h + 3]), "r"(p[8 * h + 4]),
-                           "r"(p[8 * h + 5]), "r"(p[8 * h + 6]), "r"(p[8 * h + 7])
-                           : "memory");
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: the sums of O are zero too
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (x.n > 0) {
+            tmem_ld32(tmem_base + lane_addr + 256 + t * 128 + c * 32, o);
+            tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-              reinterpret_cast<uint4*>(out + c * 32)[h] = make_uint4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            p[e] = pack2(T(), __uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          if (row_ok) {
+            if (sh.wide_out) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c * 32 + h * 16),
+                             "r"(p[8 * h]), "r"(p[8 * h + 1]), "r"(p[8 * h + 2]), "r"(p[8 * h + 3]), "r"(p[8 * h + 4]),
+                             "r"(p[8 * h + 5]), "r"(p[8 * h + 6]), "r"(p[8 * h + 7])
+                             : "memory");
+            } else {
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                reinterpret_cast<uint4*>(out + c * 32)[h] = make_uint4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+            }
           }
         }
+        if (x.n > 0) {
+          tc_fence_before();
+          mbar_arrive(&o_empty[t]);
+        }
+        if (row_ok && a.lse != nullptr)
+          a.lse[(static_cast<int64_t>(x.b) * a.heads + at.x) * a.seq_q + i_q] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
       }
-      if (row_ok && a.lse != nullptr)
-        a.lse[(static_cast<int64_t>(x.b) * a.heads + x.h) * a.seq_q + i_q] =
-            l_run == 0.f ? -INFINITY : m_run * a.scale + logf(l_run);
-      tc_fence_before();  // O may be written again once the next P is handed over
     }
   }
 
@@ -722,7 +784,8 @@ template <typename T, int D>
 void launch_tiles(const CrossAttnArgs& a, cudaStream_t s) {
   using Cfg = TileCfg<D>;
   auto kern = cross_tile_kernel<T, D>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, Cfg::kSmemBytes, allowed);
   TileMaps maps;
   TileShape sh;
   // a dimension of one entry, or a batch stride of 0, reads entry 0 alone: its stride is not used
@@ -735,8 +798,9 @@ void launch_tiles(const CrossAttnArgs& a, cudaStream_t s) {
   maps.q = map(a.q, a.seq_q, a.heads, a.q_row, a.q_batch, kQT, sh.q_shared);
   maps.k = map(a.k, a.seq_k, a.heads_kv, a.k_row, a.k_batch, kKT, sh.k_shared);
   maps.v = map(a.v, a.seq_k, a.heads_kv, a.v_row, a.v_batch, kKT, sh.v_shared);
-  sh.q_blocks = (a.seq_q + 2 * kQT - 1) / (2 * kQT);
-  const int64_t units = static_cast<int64_t>(sh.q_blocks) * a.heads * a.batch;
+  sh.q_tiles = (a.seq_q + kQT - 1) / kQT;
+  sh.pairs = static_cast<int>((static_cast<int64_t>(sh.q_tiles) * (a.heads / a.heads_kv) + 1) / 2);
+  const int64_t units = static_cast<int64_t>(sh.pairs) * a.heads_kv * a.batch;
   if (units > 0x3fffffff) throw std::runtime_error("cross_attention: too many queries");
   sh.units = static_cast<int>(units);
   sh.wide_out = reinterpret_cast<uintptr_t>(a.o) % 32 == 0 && a.o_row % 16 == 0 && a.o_batch % 16 == 0;

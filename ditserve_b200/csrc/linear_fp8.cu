@@ -429,7 +429,8 @@ template <typename T, bool kPair>
 void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   constexpr int kCtas = kPair ? 2 : 1;
   auto kern = linear_tile_kernel<T, kPair>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, kSmemBytes, allowed);
   const CUtensorMap tmX = make_tmap_u8_2d(a.x, a.M, a.K, a.ldx, kBM);
   const CUtensorMap tmW = make_tmap_u8_2d(a.w, a.N, a.K, a.ldw, bn / kCtas);
   auto at = [](const void* p, int64_t bytes, int n) {

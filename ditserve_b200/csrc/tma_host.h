@@ -5,6 +5,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -100,6 +101,17 @@ inline CUtensorMap make_tmap_out_2d(void* base, CUtensorMapDataType type, int el
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
   return map;
+}
+
+// Lets `kern` use `bytes` of shared memory on the current device: once a device, `done` holds their bits.
+template <typename Kernel>
+inline void allow_smem(Kernel kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess && dev < 64)
+    done.fetch_or(bit);
 }
 
 inline int device_sm_count() {

@@ -90,6 +90,18 @@ def kernel(name: str):
     return fn
 
 
+def launch(name: str, *args):
+    """Calls the extension entry point ``name``, which returns None where it launched nothing because its
+    arguments need another layout or are wrong; counts (and times) the launch otherwise."""
+    fn = getattr(_ext or ext(), name)
+    if _timer is not None:
+        fn = _timer.wrap(name, fn)
+    got = fn(*args)
+    if got is not None:
+        _launches[name] = _launches.get(name, 0) + 1
+    return got
+
+
 def launch_counts(reset: bool = False) -> dict[str, int]:
     """Kernel launches issued through this package since the last reset (host-side count)."""
     out = dict(_launches)
@@ -111,10 +123,13 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     buf = _status.get(idx)
     if buf is None:
+        module = ext() if available() else None
         with _lock:
             buf = _status.get(idx)
             if buf is None:
                 buf = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
+                if module is not None:
+                    module.bind_status(buf)
                 _status[idx] = buf
     return buf
 

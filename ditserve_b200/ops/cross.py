@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from ._ext import kernel, status_word, use_kernels
+from ._ext import launch, status_word, use_kernels
 
 
 def cross_attention_reference(q, k, v, heads, heads_kv=None, kv_lens=None, key_mask=None, scale=None, return_lse=False):
@@ -67,6 +67,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     place, others copied first; a context may be shared through a batch stride of 0 (``expand``).
     Returns out [B, Sq, heads * head_dim], with return_lse also the fp32 natural-log sums [B, heads, Sq]."""
     heads_kv = heads_kv or heads
+    if q.is_cuda:
+        got = launch("cross_attention", q, k, v, heads, heads_kv, kv_lens, key_mask, scale, out, return_lse)
+        if got is not None:
+            return got
     if q.dim() == 2:
         if k.dim() != 2 or v.dim() != 2 or (out is not None and out.dim() != 2):
             raise ValueError("q, k, v and out must agree in dimensions")
@@ -101,14 +105,16 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         o, lse = cross_attention_reference(q, k, v, heads, heads_kv, kv_lens, key_mask, scale, True)
         o = o if out is None else out.copy_(o)
         return (o, lse) if return_lse else o
-    o = torch.empty(B, Sq, width, device=q.device, dtype=q.dtype) if out is None else out
-    lse = torch.empty(B, heads, Sq, device=q.device, dtype=torch.float32) if return_lse else None
-    if Sk == 0:
-        o.zero_()
-        return (o, lse.fill_(-math.inf)) if return_lse else o
-    if o.numel():
-        if kv_lens is not None and kv_lens.dtype != torch.int32:
-            kv_lens = kv_lens.clamp(0, Sk).to(torch.int32)
-        kernel("cross_attention")(_strided(q), _strided(k), _strided(v), o, lse, kv_lens, key_mask, int(heads),
-                                  int(heads_kv), d, scale, status_word(q.device))
-    return (o, lse) if return_lse else o
+    # what the kernel does not take as it is: no rows, no keys, other strides, the first call on a device
+    if Sk == 0 or q.numel() == 0:
+        o = torch.zeros_like(q, memory_format=torch.contiguous_format) if out is None else out.zero_()
+        lse = torch.full((B, heads, Sq), -math.inf, device=q.device, dtype=torch.float32) if return_lse else None
+        return (o, lse) if return_lse else o
+    status_word(q.device)
+    if kv_lens is not None:
+        kv_lens = kv_lens.clamp(0, Sk).to(torch.int32).contiguous()
+    got = launch("cross_attention", _strided(q), _strided(k), _strided(v), heads, heads_kv, kv_lens, key_mask, scale, out,
+                 return_lse)
+    if got is None:
+        raise ValueError("cross_attention needs its tensors on one CUDA device and out with separate rows on 16 bytes")
+    return got

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from ._ext import kernel, status_word, use_kernels
+from ._ext import launch, status_word, use_kernels
 from .gemm import _row_gate, gelu_tanh_ref
 
 E4M3 = torch.float8_e4m3fn
@@ -87,6 +87,10 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
     y ~ q * scale[..., None], scale = max(max|y| / 448, 1e-30), and h in x's type (None without a
     residual).  The norm reads h as it is stored.  ``residual_out`` may be ``residual`` or ``x`` itself.
     A NaN or an infinity in a row makes the row's scale and q NaN."""
+    if x.is_cuda:
+        got = launch("rms_norm_quant", x, weight, residual, eps, out, scale_out, residual_out)
+        if got is not None:
+            return got
     if x.dtype not in _TYPES:
         raise ValueError("rms_norm_quant takes bf16, fp16 or fp32")
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -108,27 +112,23 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
         s = s if scale_out is None else scale_out.copy_(s)
         h = h if residual_out is None else residual_out.copy_(h)
         return q, s, h
-    x2 = x if x.dim() == 2 else x.reshape(-1, d)
-    if x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    rows = x2.shape[0]
-    q2 = empty_fp8(rows, d, x.device) if out is None else _rows_view(out, d, "out")
-    s1 = torch.empty(rows, device=x.device, dtype=torch.float32) if scale_out is None else scale_out.view(-1)
-    r2 = h2 = None
+    # what the kernel does not take as it is: columns apart, outputs in other layouts
+    x2, r2, h2 = x.reshape(-1, d), None, None
+    x2 = x2 if x2.stride(1) == 1 or d == 1 else x2.contiguous()
+    q2 = empty_fp8(x2.shape[0], d, x.device) if out is None else _rows_view(out, d, "out")
+    s1 = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
     if residual is not None:
-        r2 = residual if residual.dim() == 2 else residual.reshape(-1, d)
-        if r2.stride(1) != 1:
-            r2 = r2.contiguous()
-        h2 = torch.empty(rows, d, device=x.device, dtype=x.dtype) if residual_out is None else \
+        r2 = residual.reshape(-1, d)
+        r2 = r2 if r2.stride(1) == 1 or d == 1 else r2.contiguous()
+        h2 = torch.empty(x2.shape[0], d, device=x.device, dtype=x.dtype) if residual_out is None else \
             _rows_view(residual_out, d, "residual_out")
         if residual_out is not None and (_partial_overlap(h2, x2) or _partial_overlap(h2, r2)):
             raise ValueError("residual_out overlaps its inputs without being one of them")
-    if weight is not None and weight.stride(0) != 1:
-        weight = weight.contiguous()
-    kernel("rms_norm_quant")(x2, weight, r2, h2, q2, s1, float(eps))
-    if len(shape) == 2:
-        return (q2 if out is None else out), (s1 if scale_out is None else scale_out), h2 if residual_out is None else residual_out
-    return (q2.view(shape) if out is None else out, s1.view(shape[:-1]) if scale_out is None else scale_out,
+    weight = weight if weight is None else weight.contiguous()
+    if launch("rms_norm_quant", x2, weight, r2, eps, q2, s1, h2) is None:
+        raise ValueError("rms_norm_quant needs its tensors on one CUDA device and outputs with packed, separate rows")
+    scale = s1.view(shape[:-1]) if scale_out is None else scale_out.copy_(s1.view(shape[:-1]))
+    return (q2.view(shape) if out is None else out, scale,
             None if residual is None else (h2.view(shape) if residual_out is None else residual_out))
 
 
@@ -169,6 +169,11 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     ``out_dtype`` (bf16, fp16 or fp32; ``out`` decides if given).  ``out`` may be ``residual`` itself.
     gate is fp32 [N] or [B, N] and needs a residual; row m takes gate row m // rows_per_batch, or
     row_batch[m] (entries outside [0, B) take the nearest row)."""
+    if xq.is_cuda and act in (None, "gelu"):
+        y = launch("linear_fp8", xq, x_scale, wq, w_scale, b, act is not None, residual, gate, rows_per_batch, row_batch,
+                   out, out_dtype)
+        if y is not None:
+            return y
     if xq.dtype != E4M3 or wq.dtype != E4M3:
         raise ValueError("xq and wq must be float8_e4m3fn")
     if xq.dim() < 1 or wq.dim() != 2 or xq.shape[-1] != wq.shape[1] or wq.shape[1] == 0:
@@ -210,20 +215,19 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
             row_batch = row_batch.clamp(0, gate.shape[0] - 1)
         y = linear_fp8_reference(xq, x_scale, wq, w_scale, b, act, residual, gate, rows_per_batch, row_batch, out_dtype)
         return y if out is None else out.copy_(y)
-    x2 = _aligned_rows(xq if xq.dim() == 2 else xq.reshape(-1, K))
-    w2 = _aligned_rows(wq)
+    # what the kernel does not take as it is: rows off 16 bytes, columns apart, the first call on a device
+    status_word(xq.device)
     y2 = torch.empty(M, N, device=xq.device, dtype=out_dtype) if out is None else _rows_view(out, N, "out")
     r2 = None
     if residual is not None:
-        r2 = residual if residual.dim() == 2 else residual.reshape(-1, N)
-        if r2.stride(1) != 1:
-            r2 = r2.contiguous()
+        r2 = residual.reshape(-1, N)
+        r2 = r2 if r2.stride(1) == 1 or N == 1 else r2.contiguous()
         if out is not None and _partial_overlap(y2, r2):
             raise ValueError("out overlaps the residual without being it")
-    if b is not None and b.stride(0) != 1:
-        b = b.contiguous()
-    if gate is not None and gate.stride(1) != 1:
-        gate = gate.contiguous()
-    kernel("linear_fp8")(x2, x_scale.reshape(-1), w2, w_scale, y2, b, act is not None, r2, gate,
-                         int(rows_per_batch or max(M, 1)), row_batch, status_word(xq.device))
-    return (y2 if len(lead) == 1 else y2.view(*lead, N)) if out is None else out
+    got = launch("linear_fp8", _aligned_rows(xq.reshape(-1, K)), x_scale.reshape(-1).contiguous(), _aligned_rows(wq),
+                 w_scale.contiguous(), b if b is None else b.contiguous(), act is not None, r2,
+                 gate if gate is None or gate.stride(1) == 1 else gate.contiguous(), rows_per_batch,
+                 row_batch if row_batch is None else row_batch.contiguous(), y2, out_dtype)
+    if got is None:
+        raise ValueError("linear_fp8 needs its tensors on one CUDA device and out with packed, separate rows")
+    return y2.view(*lead, N) if out is None else out

@@ -6,9 +6,11 @@ math runs in PyTorch.  The op has no gradient of its own; ``inverse=True`` is it
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
-from ._ext import kernel, use_kernels
+from ._ext import ext, launch, use_kernels
 from .fp8 import _partial_overlap, _rows_view
 
 _POSITIONS = (torch.int64, torch.int32, torch.float32, torch.float64)
@@ -37,6 +39,13 @@ def rope_axes_reference(x, positions, dims, head_dim, theta, layout="interleaved
     return y.reshape(x.shape).to(x.dtype)
 
 
+@functools.lru_cache(maxsize=64)
+def _plan(dims: tuple, theta):
+    """The frequencies of a set of axes, or None where dims or theta are wrong (the caller says how)."""
+    thetas = [float(theta)] * len(dims) if isinstance(theta, (int, float)) else [float(t) for t in theta]
+    return ext().rope_plan([int(d) for d in dims], thetas)
+
+
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor | None = None, head_dim: int = 128,
               theta=10000.0, layout: str = "interleaved", inverse: bool = False, out: torch.Tensor | None = None,
               k_out: torch.Tensor | None = None):
@@ -48,6 +57,12 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
     position * theta^(-2j / d); theta is one number or one for each axis.  layout "interleaved" pairs
     elements (2i, 2i + 1), "half" pairs (i, i + sum(dims) / 2).  inverse turns the other way.  x and k
     (bf16, fp16 or fp32) may differ in heads.  out / k_out may be x / k themselves."""
+    if x.is_cuda and layout in ("interleaved", "half"):
+        plan = _plan(tuple(dims), theta if isinstance(theta, (int, float)) else tuple(theta))
+        if plan is not None:
+            got = launch("rope_axes", x, k, positions, plan, head_dim, layout == "half", inverse, out, k_out)
+            if got is not None:
+                return got
     dims = tuple(int(d) for d in dims)
     if not 1 <= len(dims) <= MAX_AXES or any(d <= 0 or d % 2 for d in dims):
         raise ValueError(f"dims must be 1 to {MAX_AXES} positive even numbers")
@@ -87,24 +102,24 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
                                         inverse).reshape(t.shape)
                 got.append(r if o is None else o.copy_(r))
         return got[0] if k is None else tuple(got)
-    args, got = [], []
-    for t, o in ((x, out), (k, k_out)):
+    # what the kernel does not take as it is: columns apart, several outputs to tell apart
+    t2, o2, w = [], [], [x.shape[-1], 0 if k is None else k.shape[-1]]
+    for i, (t, o) in enumerate(((x, out), (k, k_out))):
         if t is None:
-            args += [None, None]
+            t2.append(None), o2.append(None)
             continue
-        w = t.shape[-1]
-        t2 = t if t.dim() == 2 else t.reshape(-1, w)
-        if t2.stride(1) != 1:
-            t2 = t2.contiguous()
-        o2 = torch.empty(rows, w, device=x.device, dtype=x.dtype) if o is None else _rows_view(o, w, "out")
-        got.append((o2 if t.dim() == 2 else o2.view(t.shape)) if o is None else o)
-        args += [t2, o2]
+        t2.append(t.reshape(-1, w[i]))
+        if t2[i].stride(1) != 1 and w[i] > 1:
+            t2[i] = t2[i].contiguous()
+        o2.append(torch.empty(rows, w[i], device=x.device, dtype=x.dtype) if o is None else _rows_view(o, w[i], "out"))
     if rows and (out is not None or k_out is not None):
-        for o2 in (args[1], args[3]):
-            if o2 is not None and any(_partial_overlap(o2, t2) for t2 in (args[0], args[2]) if t2 is not None):
-                raise ValueError("an output overlaps an input without being it")
-        if k is not None and (args[1].data_ptr() == args[3].data_ptr() or _partial_overlap(args[1], args[3])
-                              or args[1].data_ptr() == args[2].data_ptr() or args[3].data_ptr() == args[0].data_ptr()):
+        if any(_partial_overlap(a, b) for a in o2 if a is not None for b in t2 if b is not None):
+            raise ValueError("an output overlaps an input without being it")
+        if k is not None and (o2[0].data_ptr() == o2[1].data_ptr() or _partial_overlap(o2[0], o2[1])
+                              or o2[0].data_ptr() == t2[1].data_ptr() or o2[1].data_ptr() == t2[0].data_ptr()):
             raise ValueError("the outputs of x and k must be apart")
-    kernel("rope_axes")(*args, positions, list(dims), list(theta), int(head_dim), layout == "half", bool(inverse))
-    return got[0] if k is None else tuple(got)
+    if launch("rope_axes", t2[0], t2[1], positions, _plan(dims, theta), head_dim, layout == "half", inverse, o2[0],
+              o2[1]) is None:
+        raise ValueError("rope_axes needs its tensors on one CUDA device and outputs with packed, separate rows")
+    x2 = o2[0].view(x.shape) if out is None else out
+    return x2 if k is None else (x2, o2[1].view(k.shape) if k_out is None else k_out)

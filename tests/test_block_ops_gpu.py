@@ -322,3 +322,28 @@ def test_refusals_on_the_device():
         ops.cross_attention(q, q, q, 1, kv_lens=torch.ones(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         ops.cross_attention(q, q, q, 1, out=q)
+
+
+def _to_dev(case):
+    """The CPU refusals' calls on CUDA tensors: creation functions inside them run under a default device."""
+    def run(*args):
+        with torch.device(_dev()):
+            case(*(a.to(_dev()) for a in args))
+    return run
+
+
+def test_refusals_of_the_cpu_hold_on_the_device():
+    import test_block_ops as cpu
+    marks = {f.__name__: f.pytestmark[0].args[1] for f in (cpu.test_rms_norm_quant_refusals, cpu.test_linear_fp8_refusals,
+                                                           cpu.test_rope_axes_refusals, cpu.test_cross_attention_refusals)}
+    args = {"test_rms_norm_quant_refusals": (torch.ones(4, 16, dtype=BF), torch.ones(16, dtype=BF)),
+            "test_linear_fp8_refusals": (*cpu._quantised(4, 6, 32), torch.zeros(6, dtype=BF)),
+            "test_rope_axes_refusals": (torch.ones(8, 64, dtype=BF), ops.grid_positions((2, 2, 2))),
+            "test_cross_attention_refusals": (torch.ones(2, 3, 128, dtype=BF), torch.ones(2, 5, 128, dtype=BF))}
+    before = ops.launch_counts()
+    for name, cases in marks.items():
+        for i, case in enumerate(cases):
+            with pytest.raises(ValueError):
+                _to_dev(case)(*args[name])
+                pytest.fail(f"{name}[{i}] was not refused")
+    assert ops.launch_counts() == before  # nothing ran
