@@ -254,20 +254,19 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 // the query rows that read one key head (its heads' tiles in turn), against all key tiles of the batch entry.
 //   warp 0        TMA: Q of both tiles, K one tile ahead of V
 //   warp 1        products, in the order S_A(i+1) after PV_A(i), S_B(i+1) after PV_B(i), straight on over the
-//                 end of a unit
+//                 end of a unit: the next unit's first scores are formed while this one's output leaves
 //   warp 2        puts zeros in the values of masked keys (only with lengths or a mask)
-//   warps 4..7    softmax of tile A, a row a thread; warps 8..11 of tile B
-//   warps 12..15  outputs: O / l from TMEM to memory, while the softmax goes on with the next unit
+//   warps 4..7    softmax and output of tile A, a row a thread; warps 8..11 of tile B
 // TMEM: S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B [384, 384 + D).  P is written over the first
-// half of its S as the second product's TMEM operand.  O is rescaled only when the running maximum has grown by
-// more than 2^8, P then is at most 256 and exact sums hold in fp32.
-// An encoder's context is a few key tiles long, so a unit is short: what makes the kernel fast is
-// that nothing drains between units.  Bound by the exponentials and the products about equally.
+// half of its S as the second product's TMEM operand, in two chunks of 64 keys.  O is rescaled only when the
+// running maximum has grown by more than 2^8; P then is at most 256 and exact sums hold in fp32.
+// Bound by the chain softmax, PV, next S of a tile; LATER.
 constexpr int kQT = 128, kKT = 128, kPChunks = 2;
-constexpr int kTileThreads = 512;
-// registers a thread: 512 threads start with 128; loaders and output warps give to the softmax warps
-constexpr int kRegsOther = 88, kRegsSoftmax = 168;
-static_assert(2 * kRegsOther + 2 * kRegsSoftmax <= 4 * 128, "more registers than the block starts with");
+constexpr int kTileThreads = 384;
+
+// a softmax warp stages 32 rows x 128 bytes of O at a time, from which a tile store takes them: stores of whole
+// rows by their threads took 3700 cycles of 18400 a unit of four key tiles
+constexpr int kOutBytes = 32 * 128;
 
 template <int D>
 struct TileCfg {
@@ -275,17 +274,17 @@ struct TileCfg {
   static constexpr int kQBytes = kQT * D * 2;
   static constexpr int kKvBytes = kKT * D * 2;
   static constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
-  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 2 * kQT * 8 + 1024 + 512;
+  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 8 * kOutBytes + 1024 + 512;
 };
 
 struct TileMaps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o;
 };
 
 struct TileShape {
-  int units, pairs, q_tiles;         // unit = (b * heads_kv + hk) * pairs + pair of row tiles
+  int units, tiles, group;                  // unit = (b * heads_kv + hk) * pairs + pair of a key head's row tiles
+  FastDiv pairs, heads_kv, q_tiles;
   int k_shared, v_shared, q_shared;  // batch stride 0: one entry read by all
-  int wide_out;                      // rows of o start on 32 bytes
 };
 
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
@@ -308,29 +307,25 @@ struct Unit {
 
 __device__ __forceinline__ Unit unit_of(const CrossAttnArgs& a, const TileShape& sh, int u) {
   Unit x;
-  const int bh = u / sh.pairs;
-  x.pair = u - bh * sh.pairs;
-  x.b = bh / a.heads_kv;
+  const int bh = sh.pairs.div(u);
+  x.pair = u - bh * sh.pairs.d;
+  x.b = sh.heads_kv.div(bh);
   x.hk = bh - x.b * a.heads_kv;
   x.n = (valid_keys(a, x.b) + kKT - 1) / kKT;
-  x.two = 2 * x.pair + 1 < sh.q_tiles * (a.heads / a.heads_kv);
+  x.two = 2 * x.pair + 1 < sh.tiles;
   return x;
 }
 
 // head and first query of tile t of a unit
 __device__ __forceinline__ int2 tile_of(const CrossAttnArgs& a, const TileShape& sh, const Unit& x, int t) {
-  const int i = 2 * x.pair + t, g = i / sh.q_tiles;
-  return make_int2(x.hk * (a.heads / a.heads_kv) + g, (i - g * sh.q_tiles) * kQT);
+  const int i = 2 * x.pair + t, g = sh.q_tiles.div(i);
+  return make_int2(x.hk * sh.group + g, (i - g * sh.q_tiles.d) * kQT);
 }
 
-template <int kRegs>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
-template <int kRegs>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
-
-// One key tile of one unit; walks a CTA's units in order, leaving out those without keys.
+// One key tile of one unit; walks a CTA's units in order, leaving out those without keys.  base + j counts the key
+// tiles so far: the place in the K and V rings.
 struct Step {
-  int u, j = 0;
+  int u, j = 0, base = 0;
   Unit x;
   __device__ __forceinline__ bool settle(const CrossAttnArgs& a, const TileShape& sh) {
     for (; u < sh.units; u += gridDim.x) {
@@ -342,6 +337,7 @@ struct Step {
   __device__ __forceinline__ bool advance(const CrossAttnArgs& a, const TileShape& sh) {
     if (++j < x.n) return true;
     j = 0;
+    base += x.n;
     u += gridDim.x;
     return settle(a, sh);
   }
@@ -365,8 +361,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * Cfg::kQBytes;
   uint8_t* sV = sK + ST * Cfg::kKvBytes;
-  float2* row_ml = reinterpret_cast<float2*>(sV + ST * Cfg::kKvBytes);  // [2][128] maximum and sum of a finished row
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(row_ml + 2 * kQT);     // [2] a tile
+  uint8_t* sOut = sV + ST * Cfg::kKvBytes;                               // [8 warps]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sOut + 8 * kOutBytes);  // [2] a tile
   uint64_t* q_empty = q_full + 2;
   uint64_t* k_full = q_empty + 2;   // [ST]
   uint64_t* k_empty = k_full + ST;
@@ -376,9 +372,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* s_full = v_empty + ST;           // [2]
   uint64_t* p_full = s_full + 2;             // [2][kPChunks]
   uint64_t* pv_done = p_full + 2 * kPChunks;  // [2]
-  uint64_t* l_full = pv_done + 2;   // [2] row_ml written
-  uint64_t* o_empty = l_full + 2;   // [2] O and row_ml read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -390,9 +384,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&pv_done[i], 1);
-      mbar_init(&l_full[i], 128);
-      mbar_init(&o_empty[i], 128);
     }
+    for (int i = 0; i < 2 * kPChunks; ++i) mbar_init(&p_full[i], 4);  // one arrival a warp
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -400,7 +393,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&v_ready[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < 2 * kPChunks; ++i) mbar_init(&p_full[i], 128);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -411,7 +403,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp < 4) {
-    regs_dec<kRegsOther>();
     if (warp == 0) {
       if (lane == 0) {
         // ---------------- TMA ----------------
@@ -450,93 +441,82 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         while (ok) {
           Step next = cur;
           const bool more = next.advance(a, sh);
-          if (more) {
-            if (next.j == 0 && !load_q(next.x)) break;
-            if (!load_kv(next, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412)) break;
-          }
-          if (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
+          // at a unit's end its last V comes before the next unit's Q, which waits for the last scores
+          const bool fresh = more && next.j == 0;
+          if (fresh && (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413) || !load_q(next.x))) break;
+          if (more && !load_kv(next, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412)) break;
+          if (!fresh && !load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
           cur = next;
           ok = more;
         }
       }
     } else if (warp == 1) {
-      if (lane == 0) {
-        // ---------------- products ----------------
-        constexpr uint32_t idesc_s = kBf16 ? umma_idesc_bf16(kQT, kKT, false) : umma_idesc_fp16(kQT, kKT, false);
-        constexpr uint32_t idesc_o = kBf16 ? umma_idesc_bf16(kQT, D, true) : umma_idesc_fp16(kQT, D, true);
-        int q_count[2] = {0, 0}, p_count[2] = {0, 0}, o_count[2] = {0, 0}, kc = 0, vc = 0;
-        uint64_t* v_go = masked_kv ? v_ready : v_full;
-        // S_t = Q_t K^T of step s, whose K is the kc-th
-        auto issue_s = [&](int t, const Step& s) -> bool {
-          if (s.j == 0) {
-            if (!mbar_wait(&q_full[t], q_count[t] & 1, abort_flag, a.status, 420 + t)) return false;
-            ++q_count[t];
-          }
-          const int st = kc % ST;
-          if (t == 0) {
-            if (!mbar_wait(&k_full[st], (kc / ST) & 1, abort_flag, a.status, 422)) return false;
-          }
-          tc_fence_after();
-  #pragma unroll
+      // ---------------- products (the whole warp walks the loop, one lane issues) ----------------
+      const bool one = elect_sync();
+      constexpr uint32_t idesc_s = kBf16 ? umma_idesc_bf16(kQT, kKT, false) : umma_idesc_fp16(kQT, kKT, false);
+      constexpr uint32_t idesc_o = kBf16 ? umma_idesc_bf16(kQT, D, true) : umma_idesc_fp16(kQT, D, true);
+      constexpr uint32_t kHi = umma_desc_hi_sw128(1024);
+      const uint32_t q_lo = umma_desc_lo(smem_u32(sQ), 16), k_lo = umma_desc_lo(smem_u32(sK), 16);
+      const uint32_t v_lo = umma_desc_lo(smem_u32(sV), kKT * 128);  // 64-value blocks of V lie a tile's rows apart
+      uint64_t* v_go = masked_kv ? v_ready : v_full;
+      int units[2] = {0, 0}, steps[2] = {0, 0};
+      // S_t = Q_t K^T of a step
+      auto issue_s = [&](int t, const Step& s) -> bool {
+        const int i = s.base + s.j, st = i % ST;
+        if (s.j == 0) {
+          if (!mbar_wait_warp(&q_full[t], units[t] & 1, abort_flag, a.status, 420 + t)) return false;
+          ++units[t];
+        }
+        if (t == 0 && !mbar_wait_warp(&k_full[st], (i / ST) & 1, abort_flag, a.status, 422)) return false;
+        tc_fence_after();
+        if (one) {
+          const uint32_t q_at = q_lo + t * (Cfg::kQBytes >> 4), k_at = k_lo + st * (Cfg::kKvBytes >> 4);
+#pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kQT * 128) + (kk & 3) * 32;
-            const uint64_t da = umma_desc_sw128(smem_u32(sQ + t * Cfg::kQBytes) + off, 16, 1024);
-            const uint64_t db = umma_desc_sw128(smem_u32(sK + st * Cfg::kKvBytes) + off, 16, 1024);
-            umma_bf16_ss(tmem_base + t * kKT, da, db, idesc_s, kk != 0);
+            const uint32_t off = ((kk >> 2) * (kQT * 128) + (kk & 3) * 32) >> 4;
+            umma_f16_ss(tmem_base + t * kKT, q_at + off, kHi, k_at + off, kHi, idesc_s, kk != 0);
           }
           umma_commit(&s_full[t]);
+          if (t == 1 || !s.x.two) umma_commit(&k_empty[st]);
           if (s.j + 1 == s.x.n) umma_commit(&q_empty[t]);
-          return true;
-        };
-        // O_t (+)= P_t V of step s, whose V is the vc-th
-        auto issue_pv = [&](int t, const Step& s) -> bool {
-          const uint32_t v_base = smem_u32(sV + (vc % ST) * Cfg::kKvBytes);
-          constexpr int kPer = kKT / 16 / kPChunks;
-          if (s.j == 0) {  // the unit before has been written out
-            if (!mbar_wait(&o_empty[t], (o_count[t] & 1) ^ 1, abort_flag, a.status, 426 + t)) return false;
-            ++o_count[t];
-          }
-  #pragma unroll
-          for (int c = 0; c < kPChunks; ++c) {
-            if (!mbar_wait(&p_full[t * kPChunks + c], p_count[t] & 1, abort_flag, a.status, 424 + t)) return false;
-            tc_fence_after();
-  #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const int kk = c * kPer + i;
-              const uint64_t db = umma_desc_sw128(v_base + kk * (16 * 128), kKT * 128, 1024);
-              umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * kKT + kk * 8, db, idesc_o, (s.j | kk) != 0);
-            }
-          }
-          ++p_count[t];
-          umma_commit(&pv_done[t]);
-          return true;
-        };
-        Step cur;
-        cur.u = blockIdx.x;
-        bool ok = cur.settle(a, sh);
-        if (ok) {
-          ok = issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
-          umma_commit(&k_empty[kc % ST]);
-          ++kc;
         }
-        while (ok) {
-          Step next = cur;
-          const bool more = next.advance(a, sh);
-          if (!mbar_wait(&v_go[vc % ST], (vc / ST) & 1, abort_flag, a.status, 423)) break;
+        return true;
+      };
+      // O_t (+)= P_t V of a step
+      auto issue_pv = [&](int t, const Step& s) -> bool {
+        const int i = s.base + s.j, st = i % ST;
+        const uint32_t v_at = v_lo + st * (Cfg::kKvBytes >> 4);
+        if (t == 0 && !mbar_wait_warp(&v_go[st], (i / ST) & 1, abort_flag, a.status, 423)) return false;
+#pragma unroll
+        for (int c = 0; c < kPChunks; ++c) {
+          if (!mbar_wait_warp(&p_full[t * kPChunks + c], steps[t] & 1, abort_flag, a.status, 424 + t)) return false;
           tc_fence_after();
-          if (!issue_pv(0, cur)) break;
-          if (more && !issue_s(0, next)) break;
-          if (cur.x.two && !issue_pv(1, cur)) break;
-          umma_commit(&v_empty[vc % ST]);
-          ++vc;
-          if (more) {
-            if (next.x.two && !issue_s(1, next)) break;
-            umma_commit(&k_empty[kc % ST]);
-            ++kc;
+          constexpr int kPer = kKT / 16 / kPChunks;
+          if (one) {
+#pragma unroll
+            for (int kk = c * kPer; kk < (c + 1) * kPer; ++kk)
+              umma_f16_ts(tmem_base + 256 + t * 128, tmem_base + t * kKT + kk * 8, v_at + kk * (16 * 128 / 16), kHi, idesc_o,
+                          (s.j | kk) != 0);
           }
-          cur = next;
-          ok = more;
         }
+        ++steps[t];
+        if (one) {
+          umma_commit(&pv_done[t]);
+          if (t == 1 || !s.x.two) umma_commit(&v_empty[st]);
+        }
+        return true;
+      };
+      Step cur;
+      cur.u = blockIdx.x;
+      bool ok = cur.settle(a, sh) && issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
+      while (ok) {
+        Step next = cur;
+        const bool more = next.advance(a, sh);
+        if (!issue_pv(0, cur) || (more && !issue_s(0, next))) break;
+        if (cur.x.two && !issue_pv(1, cur)) break;
+        if (more && next.x.two && !issue_s(1, next)) break;
+        cur = next;
+        ok = more;
       }
     } else if (warp == 2) {
       if (masked_kv) {
@@ -568,9 +548,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
     }
-  } else if (warp < 12) {
-    regs_inc<kRegsSoftmax>();
-    // ---------------- softmax of tile t ----------------
+  } else {
+    // ---------------- softmax and output of tile t ----------------
     const int t = (warp >> 2) - 1;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -579,12 +558,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t o_col = tmem_base + lane_addr + 256 + t * 128;
     const float sl2 = a.scale * kLog2e;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
+    auto hand_over = [&](int c) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t * kPChunks + c]);
+    };
+    uint8_t* out = sOut + (warp - 4) * kOutBytes;
     int step = 0;  // key tiles of tile t so far: the phase of its barriers
-    int done = 0;  // units of tile t so far
     bool ok = true;
     for (int u = blockIdx.x; ok && u < sh.units; u += gridDim.x) {
       const Unit x = unit_of(a, sh, u);
-      if (x.n == 0 || (t == 1 && !x.two)) continue;
+      if (t == 1 && !x.two) continue;
       const int valid = valid_keys(a, x.b);
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < x.n; ++j, ++step) {
@@ -644,125 +629,79 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         // a rescale of O has to come before the products that follow; without one the chunks of P go at once
         const bool rescale = j > 0 && __any_sync(0xffffffffu, need);
-        constexpr int kChunkCh = kKT / 8 / kPChunks;
-        int signalled = 0;
-        uint32_t pk8[8];
+        constexpr int kChunk = kKT / kPChunks;
+        uint32_t pk[8];
 #pragma unroll
-        for (int ch = 0; ch < kKT / 8; ++ch) {
-          float e8[8];
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const int c = ch * 8 + e;
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2x2, negx2), x0, x1);
-            e8[e] = ex2_approx(x0);
-            e8[e + 1] = ex2_approx(x1);
-            ls[e] += e8[e];
-            ls[e + 1] += e8[e + 1];
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pk8[(ch & 1) * 4 + e] = pack2(T(), e8[2 * e], e8[2 * e + 1]);
-          if (ch & 1) tmem_st8(s_col + (ch >> 1) * 8, pk8);
-          if (!rescale && (ch + 1) % kChunkCh == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[t * kPChunks + (ch + 1) / kChunkCh - 1]);
-            signalled = ch + 1;
-          }
+        for (int c = 0; c < kKT; c += 2) {
+          float x0, x1;
+          const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2x2, negx2);
+          f2_unpack(x2, x0, x1);
+          x0 = ex2_approx(x0);
+          x1 = ex2_approx(x1);
+          ls[c & 7] += x0;
+          ls[(c & 7) + 1] += x1;
+          pk[(c / 2) & 7] = pack2(T(), x0, x1);
+          if ((c & 15) == 14) tmem_st8(s_col + (c >> 4) * 8, pk);
+          if ((c + 2) % kChunk == 0 && c + 2 < kKT && !rescale) hand_over((c + 2) / kChunk - 1);
         }
         l_run += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
         if (rescale) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
-            tmem_ld32(o_col + c * 32, o);
+            tmem_ld32(o_col + c, o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(o_col + c * 32, o);
+            tmem_st32(o_col + c, o);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          for (int c = signalled / kChunkCh; c < kPChunks; ++c) mbar_arrive(&p_full[t * kPChunks + c]);
+          for (int c = 0; c < kPChunks - 1; ++c) hand_over(c);
         }
+        hand_over(kPChunks - 1);
       }
       if (!ok) break;
-      // the output warps have read the unit before
-      if (!mbar_wait_warp(&o_empty[t], (done & 1) ^ 1, abort_flag, a.status, 444 + t)) break;
-      ++done;
-      row_ml[t * kQT + row] = make_float2(m_run, l_run);
-      mbar_arrive(&l_full[t]);
-    }
-  } else {
-    regs_dec<kRegsOther>();
-    // ---------------- outputs ----------------
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    int step[2] = {0, 0}, done[2] = {0, 0};
-    bool ok = true;
-    for (int u = blockIdx.x; ok && u < sh.units; u += gridDim.x) {
-      const Unit x = unit_of(a, sh, u);
-      for (int t = 0; t < (x.two ? 2 : 1); ++t) {
-        const int2 at = tile_of(a, sh, x, t);
-        const int i_q = at.y + row;
-        const bool row_ok = i_q < a.seq_q;
-        T* out = reinterpret_cast<T*>(a.o) + x.b * a.o_batch + static_cast<int64_t>(i_q) * a.o_row + at.x * D;
-        float m = -INFINITY, l = 0.f;
-        if (x.n > 0) {
-          if (!mbar_wait_warp(&l_full[t], done[t] & 1, abort_flag, a.status, 450 + t)) {
-            ok = false;
-            break;
-          }
-          ++done[t];
-          const float2 ml = row_ml[t * kQT + row];
-          m = ml.x;
-          l = ml.y;
-          step[t] += x.n;
-          if (!mbar_wait_warp(&pv_done[t], (step[t] - 1) & 1, abort_flag, a.status, 452 + t)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: the sums of O are zero too
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          if (x.n > 0) {
-            tmem_ld32(tmem_base + lane_addr + 256 + t * 128 + c * 32, o);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0;
-          }
-          uint32_t p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            p[e] = pack2(T(), __uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-          if (row_ok) {
-            if (sh.wide_out) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c * 32 + h * 16),
-                             "r"(p[8 * h]), "r"(p[8 * h + 1]), "r"(p[8 * h + 2]), "r"(p[8 * h + 3]), "r"(p[8 * h + 4]),
-                             "r"(p[8 * h + 5]), "r"(p[8 * h + 6]), "r"(p[8 * h + 7])
-                             : "memory");
-            } else {
-#pragma unroll
-              for (int h = 0; h < 4; ++h)
-                reinterpret_cast<uint4*>(out + c * 32)[h] = make_uint4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
-            }
-          }
-        }
-        if (x.n > 0) {
-          tc_fence_before();
-          mbar_arrive(&o_empty[t]);
-        }
-        if (row_ok && a.lse != nullptr)
-          a.lse[(static_cast<int64_t>(x.b) * a.heads + at.x) * a.seq_q + i_q] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+      const int2 at = tile_of(a, sh, x, t);
+      const int i_q = at.y + row;
+      const bool row_ok = i_q < a.seq_q;
+      const float inv = m_run == -INFINITY ? 0.f : 1.f / l_run;  // no key: zeros
+      if (x.n > 0) {
+        if (!mbar_wait_warp(&pv_done[t], (step - 1) & 1, abort_flag, a.status, 444 + t)) break;
+        tc_fence_after();
       }
+      uint32_t o[D];
+      if (x.n > 0) {
+#pragma unroll
+        for (int c = 0; c < D; c += 32) tmem_ld32(o_col + c, *reinterpret_cast<uint32_t(*)[32]>(&o[c]));
+        tmem_wait_ld();
+        tc_fence_before();  // O may be written again once the next P is handed over
+      } else {
+#pragma unroll
+        for (int c = 0; c < D; ++c) o[c] = 0;
+      }
+#pragma unroll
+      for (int c = 0; c < D; c += 64) {
+        if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {  // 16-byte pieces in the 128-byte swizzle's places
+          uint32_t p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            p[e] = pack2(T(), __uint_as_float(o[c + 8 * q + 2 * e]) * inv, __uint_as_float(o[c + 8 * q + 2 * e + 1]) * inv);
+          *reinterpret_cast<uint4*>(out + lane * 128 + ((q ^ (lane & 7)) * 16)) = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (at.y + quarter * 32 < a.seq_q) tma_store_3d(&maps.o, at.x * D + c, at.y + quarter * 32, x.b, out);
+          tma_store_commit();
+        }
+      }
+      if (row_ok && a.lse != nullptr)
+        a.lse[(static_cast<int64_t>(x.b) * a.heads + at.x) * a.seq_q + i_q] =
+            m_run == -INFINITY ? -INFINITY : m_run * a.scale + logf(l_run);
     }
+    if (lane == 0) tma_store_wait_all();
   }
 
   tc_fence_before();
@@ -798,12 +737,19 @@ void launch_tiles(const CrossAttnArgs& a, cudaStream_t s) {
   maps.q = map(a.q, a.seq_q, a.heads, a.q_row, a.q_batch, kQT, sh.q_shared);
   maps.k = map(a.k, a.seq_k, a.heads_kv, a.k_row, a.k_batch, kKT, sh.k_shared);
   maps.v = map(a.v, a.seq_k, a.heads_kv, a.v_row, a.v_batch, kKT, sh.v_shared);
-  sh.q_tiles = (a.seq_q + kQT - 1) / kQT;
-  sh.pairs = static_cast<int>((static_cast<int64_t>(sh.q_tiles) * (a.heads / a.heads_kv) + 1) / 2);
-  const int64_t units = static_cast<int64_t>(sh.pairs) * a.heads_kv * a.batch;
+  const uint64_t width = static_cast<uint64_t>(a.heads) * D;
+  const uint64_t o_row = a.seq_q == 1 ? width : a.o_row;
+  maps.o = make_tmap_16bit_3d(a.o, a.batch, a.seq_q, width, o_row, a.batch == 1 ? o_row * a.seq_q : a.o_batch, 32);
+  const int q_tiles = (a.seq_q + kQT - 1) / kQT;
+  sh.group = a.heads / a.heads_kv;
+  sh.tiles = q_tiles * sh.group;
+  const int pairs = (sh.tiles + 1) / 2;
+  const int64_t units = static_cast<int64_t>(pairs) * a.heads_kv * a.batch;
   if (units > 0x3fffffff) throw std::runtime_error("cross_attention: too many queries");
   sh.units = static_cast<int>(units);
-  sh.wide_out = reinterpret_cast<uintptr_t>(a.o) % 32 == 0 && a.o_row % 16 == 0 && a.o_batch % 16 == 0;
+  sh.pairs = FastDiv(pairs);
+  sh.heads_kv = FastDiv(a.heads_kv);
+  sh.q_tiles = FastDiv(q_tiles);
   const int sms = device_sm_count();
   kern<<<units < sms ? sh.units : sms, kTileThreads, Cfg::kSmemBytes, s>>>(maps, a, sh);
 }

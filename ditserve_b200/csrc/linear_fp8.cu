@@ -286,35 +286,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     producer_done:;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {  // the whole warp walks the loop, one lane issues
+      const bool one = elect_sync();
+      constexpr uint32_t kHi = umma_desc_hi_sw128(1024);
+      const uint32_t ring_lo = umma_desc_lo(smem_u32(ring), 16);
       const uint32_t idesc = umma_idesc_e4m3(kCtas * kBM, sh.bn);
       int stage = 0, local = 0;
       uint32_t phase = 0;
       for (int tile = first; tile < tiles; tile += step, ++local) {
         const int acc = local & 1;
-        if (!mbar_wait(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, a.status, 311)) goto mma_done;
+        if (!mbar_wait_warp(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, a.status, 311)) goto mma_done;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * kMaxBn;
         for (int kb = 0; kb < sh.num_k; ++kb) {
-          if (!mbar_wait(&full[stage], phase, abort_flag, a.status, 312)) goto mma_done;
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag, a.status, 312)) goto mma_done;
           tc_fence_after();
-          const uint64_t da = umma_desc_sw128(smem_u32(ring + stage * sh.stage_bytes), 16, 1024);
-          const uint64_t db = umma_desc_sw128(smem_u32(ring + stage * sh.stage_bytes + kABytes), 16, 1024);
+          const uint32_t a_lo = ring_lo + stage * (sh.stage_bytes >> 4), b_lo = a_lo + (kABytes >> 4);
+          if (one) {
 #pragma unroll
-          for (int k = 0; k < kBK / 32; ++k) {
-            // 32 bytes onwards inside the swizzle atom: 2 in the address field
-            if constexpr (kPair) umma_e4m3_ss_pair(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
-            else umma_e4m3_ss(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            for (int k = 0; k < kBK / 32; ++k) {
+              // 32 bytes onwards inside the swizzle atom: 2 in the address field
+              if constexpr (kPair) umma_f8_ss_pair(d, a_lo + 2 * k, kHi, b_lo + 2 * k, kHi, idesc, (kb | k) != 0);
+              else umma_f8_ss(d, a_lo + 2 * k, kHi, b_lo + 2 * k, kHi, idesc, (kb | k) != 0);
+            }
+            if constexpr (kPair) umma_commit_pair(&empty[stage]);
+            else umma_commit(&empty[stage]);
           }
-          if constexpr (kPair) umma_commit_pair(&empty[stage]);
-          else umma_commit(&empty[stage]);
           if (++stage == ST) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if constexpr (kPair) umma_commit_pair(&acc_full[acc]);
-        else umma_commit(&acc_full[acc]);
+        if (one) {
+          if constexpr (kPair) umma_commit_pair(&acc_full[acc]);
+          else umma_commit(&acc_full[acc]);
+        }
       }
     mma_done:;
     }
