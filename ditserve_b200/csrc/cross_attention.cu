@@ -32,32 +32,38 @@ __device__ __forceinline__ bool key_allowed(const CrossAttnArgs& a, int b, int j
   return j < valid && (a.key_mask == nullptr || a.key_mask[b * a.mask_row + j * a.mask_col] != 0);
 }
 
-// Few queries: a cluster of up to 8 blocks takes 16 query rows of one key head (a row is a query of
-// one of the heads that share the key head) and splits the keys over its warps, 16 at a time; their
-// maxima, sums and outputs are joined in shared memory, then over the cluster.  K and V go from global
-// memory straight to the products' operands in 16-byte pieces: bound by latency, then HBM.
-constexpr int kFewWarps = 4;
+// Few queries: a cluster of up to 8 blocks takes 16 query rows of one key head (a row is a query of one of the heads
+// that share the key head) and splits the keys over its warps, 16 at a time.  K and V go from global memory
+// straight to the products' operands in 16-byte pieces; a warp's maximum, sum and output are joined with the
+// others' through shared memory, then each row with the other blocks' in the block that finishes it: partials are
+// pushed there, one cluster barrier behind the pushes, sums in a fixed order.  Bound by latency:
+// one query of 2 x 12 heads over 512 keys takes 5.2 us (8.1 with the warps adding in turn and remote reads).
+constexpr int kFewWarps = 8, kFewThreads = 32 * kFewWarps, kFewRows = 16;
 
 template <int D>
 struct FewSmem {
-  float o[16][D + 4];
-  float m[16], l[16];
-  float wm[kFewWarps][16], wl[kFewWarps][16];
+  float o[kFewWarps][kFewRows][D + 4];
+  float m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
+  float in[kFewRows][D + 4];  // [source block][row / split]: the cluster's partials of the rows finished here
+  float2 in_ml[kFewRows];
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs a, int split) {
-  __shared__ FewSmem<D> sm;
+__global__ void __launch_bounds__(kFewThreads) cross_few_kernel(CrossAttnArgs a, int split) {
+  extern __shared__ __align__(16) uint8_t few_smem[];
+  FewSmem<D>& sm = *reinterpret_cast<FewSmem<D>*>(few_smem);
+  cg::cluster_group cluster = cg::this_cluster();
+  if (split > 1) cluster.barrier_arrive();  // waited for below: no push before all blocks have started
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int part = blockIdx.x % split;  // the cluster's blocks are neighbours in x
-  const int rows0 = blockIdx.x / split * 16;
+  const int rows0 = blockIdx.x / split * kFewRows;
   const int hk = blockIdx.y, b = blockIdx.z;
   const int group = a.heads / a.heads_kv;
   const int rows = a.seq_q * group;
-  const int valid = valid_keys(a, b);
   const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_batch;
   const T* k = reinterpret_cast<const T*>(a.k) + b * a.k_batch + hk * D;
   const T* v = reinterpret_cast<const T*>(a.v) + b * a.v_batch + hk * D;
+  const int valid = valid_keys(a, b);
   // query operands: lane (g, t) holds elements t * 8 .. t * 8 + 7 of every 32 of rows g and g + 8
   uint4 qa[D / 32], qb[D / 32];
   {
@@ -74,31 +80,37 @@ __global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const float sl2 = a.scale * kLog2e;
   const int stride = split * kFewWarps * 16;
-  for (int j0 = (part * kFewWarps + warp) * 16; j0 < valid; j0 += stride) {
-    float s[2][4] = {};
-    // V of this lane's four keys (2t, 2t + 1, 2t + 8, 2t + 9), zero where masked
-    uint4 vv[4][D / 64];
+  for (int j0 = (part * kFewWarps + warp) * 16; j0 < a.seq_k; j0 += stride) {
+    // all loads of the 16 keys first, whatever the lengths say: keys behind the last are read as the last
+    uint4 kk[2][D / 32], vv[4][D / 64];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const T* row = k + static_cast<int64_t>(min(j0 + n * 8 + g, a.seq_k - 1)) * a.k_row + t * 8;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) kk[n][i] = *reinterpret_cast<const uint4*>(row + i * 32);
+    }
+    // V of this lane's four keys (2t, 2t + 1, 2t + 8, 2t + 9)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T* row = v + static_cast<int64_t>(min(j0 + 2 * t + (i & 1) + (i >> 1) * 8, a.seq_k - 1)) * a.v_row + g * 8;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) vv[i][c] = *reinterpret_cast<const uint4*>(row + c * 64);
+    }
     bool ok[2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + 2 * t + (i & 1) + (i >> 1) * 8;
-      const bool on = key_allowed(a, b, j, valid);
-      ok[i >> 1][i & 1] = on;
-      const T* row = v + static_cast<int64_t>(min(j, valid - 1)) * a.v_row + g * 8;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        vv[i][c] = on ? *reinterpret_cast<const uint4*>(row + c * 64) : make_uint4(0, 0, 0, 0);
+      ok[i >> 1][i & 1] = j < a.seq_k && key_allowed(a, b, j, valid);
     }
+    if (j0 >= valid) break;
+    float s[2][4] = {};
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const T* row = k + static_cast<int64_t>(min(j0 + n * 8 + g, valid - 1)) * a.k_row + t * 8;
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        const uint4 u = *reinterpret_cast<const uint4*>(row + i * 32);
-        mma16816(T(), s[n], qa[i].x, qb[i].x, qa[i].y, qb[i].y, u.x, u.y);
-        mma16816(T(), s[n], qa[i].z, qb[i].z, qa[i].w, qb[i].w, u.z, u.w);
+        mma16816(T(), s[n], qa[i].x, qb[i].x, qa[i].y, qb[i].y, kk[n][i].x, kk[n][i].y);
+        mma16816(T(), s[n], qa[i].z, qb[i].z, qa[i].w, qb[i].w, kk[n][i].z, kk[n][i].w);
       }
-    }
     float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -117,7 +129,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs
     const float n0 = max_nan(m0, x0), n1 = max_nan(m1, x1);
     // nothing allowed so far: subtract zero, every p is 2^-inf = 0
     const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-    const float c0 = exp2f(m0 - b0), c1 = exp2f(m1 - b1);
+    const float c0 = ex2_approx(m0 - b0), c1 = ex2_approx(m1 - b1);
     m0 = n0;
     m1 = n1;
     l0 *= c0;
@@ -126,8 +138,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        s[n][e] = exp2f(s[n][e] - b0);
-        s[n][2 + e] = exp2f(s[n][2 + e] - b1);
+        s[n][e] = ex2_approx(s[n][e] - b0);
+        s[n][2 + e] = ex2_approx(s[n][2 + e] - b1);
         l0 += s[n][e];
         l1 += s[n][2 + e];
       }
@@ -140,6 +152,12 @@ __global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs
     }
     const uint32_t p0 = pack2(T(), s[0][0], s[0][1]), p1 = pack2(T(), s[0][2], s[0][3]);
     const uint32_t p2 = pack2(T(), s[1][0], s[1][1]), p3 = pack2(T(), s[1][2], s[1][3]);
+    // a masked key's value never meets a product, whatever its slot holds
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        if (!ok[i >> 1][i & 1]) vv[i][c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
       const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][c]);
@@ -162,82 +180,108 @@ __global__ void __launch_bounds__(32 * kFewWarps) cross_few_kernel(CrossAttnArgs
     l1 += __shfl_xor_sync(0xffffffffu, l1, d);
   }
   if (t == 0) {
-    sm.wm[warp][g] = m0;
-    sm.wm[warp][g + 8] = m1;
-    sm.wl[warp][g] = l0;
-    sm.wl[warp][g + 8] = l1;
+    sm.m[warp][g] = m0;
+    sm.m[warp][g + 8] = m1;
+    sm.l[warp][g] = l0;
+    sm.l[warp][g + 8] = l1;
   }
-  for (int i = threadIdx.x; i < 16 * (D + 4); i += 32 * kFewWarps) (&sm.o[0][0])[i] = 0.f;
-  __syncthreads();
-  if (threadIdx.x < 16) {
-    float m = -INFINITY;
+  const int here = min(kFewRows, rows - rows0);  // rows of this tile
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) m = max_nan(m, sm.wm[w][threadIdx.x]);
-    float l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-      const float x = m == -INFINITY ? 0.f : exp2f(sm.wm[w][threadIdx.x] - m);
-      l += x * sm.wl[w][threadIdx.x];
-      sm.wl[w][threadIdx.x] = x;  // from here on the warp's factor
+  for (int i = 0; i < D / 8; ++i) {
+    const int col = (i >> 3) * 64 + (i & 7) + 16 * t;
+    if (g < here) {
+      sm.o[warp][g][col] = o[i][0];
+      sm.o[warp][g][col + 8] = o[i][1];
     }
-    sm.m[threadIdx.x] = m;
-    sm.l[threadIdx.x] = l;
+    if (g + 8 < here) {
+      sm.o[warp][g + 8][col] = o[i][2];
+      sm.o[warp][g + 8][col + 8] = o[i][3];
+    }
   }
   __syncthreads();
-  // the warps add in turn: the order of the sums is fixed
-  for (int w = 0; w < kFewWarps; ++w) {
-    if (warp == w) {
-      const float f0 = sm.wl[w][g], f1 = sm.wl[w][g + 8];
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const int col = (i >> 3) * 64 + (i & 7);
-        sm.o[g][col + 16 * t] += f0 * o[i][0];
-        sm.o[g][col + 16 * t + 8] += f0 * o[i][1];
-        sm.o[g + 8][col + 16 * t] += f1 * o[i][2];
-        sm.o[g + 8][col + 16 * t + 8] += f1 * o[i][3];
-      }
-    }
-    __syncthreads();
-  }
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  // every block of the cluster finishes its share of the rows
-  for (int i = part * 32 * kFewWarps + threadIdx.x; i < 16 * (D / 8); i += split * 32 * kFewWarps) {
-    const int r = i / (D / 8), c = i % (D / 8) * 8;
-    const int row = rows0 + r;
-    if (row >= rows) continue;
-    float m = -INFINITY;
-    for (int p = 0; p < split; ++p) m = max_nan(m, cluster.map_shared_rank(&sm, p)->m[r]);
-    float l = 0.f, f[8] = {};
-    for (int p = 0; p < split; ++p) {
-      const FewSmem<D>* other = cluster.map_shared_rank(&sm, p);
-      const float x = m == -INFINITY ? 0.f : exp2f(other->m[r] - m);
-      l += x * other->l[r];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += x * other->o[r][c + e];
-    }
+  auto finish = [&](int r, int c, float m, float l, float4 f) {
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= inv;
-    const int i_q = row / group, h = hk * group + row % group;
-    store_vec<T, 8>(reinterpret_cast<T*>(a.o) + b * a.o_batch + i_q * a.o_row + h * D + c, f);
+    const int row = rows0 + r, i_q = row / group, h = hk * group + row % group;
+    uint2 w = make_uint2(pack2(T(), f.x * inv, f.y * inv), pack2(T(), f.z * inv, f.w * inv));
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o) + b * a.o_batch + i_q * a.o_row + h * D + c) = w;
     if (c == 0 && a.lse != nullptr)
       a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.seq_q + i_q] = (m + log2f(l)) * 0.6931471805599453f;
+  };
+  if (split > 1) cluster.barrier_wait();
+  for (int i = threadIdx.x; i < here * (D / 4); i += kFewThreads) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) m = max_nan(m, sm.m[w][r]);
+    float l = 0.f;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float x = m == -INFINITY ? 0.f : ex2_approx(sm.m[w][r] - m);
+      const float4 p = *reinterpret_cast<const float4*>(&sm.o[w][r][c]);
+      l += x * sm.l[w][r];
+      f.x += x * p.x;
+      f.y += x * p.y;
+      f.z += x * p.z;
+      f.w += x * p.w;
+    }
+    if (split == 1) {
+      finish(r, c, m, l, f);
+    } else {
+      FewSmem<D>* to = cluster.map_shared_rank(&sm, r % split);
+      const int slot = part * (kFewRows / split) + r / split;
+      *reinterpret_cast<float4*>(&to->in[slot][c]) = f;
+      if (c == 0) to->in_ml[slot] = make_float2(m, l);
+    }
   }
-  cluster.sync();  // no block leaves while another reads its shared memory
+  if (split == 1) return;
+  cluster.sync();
+  for (int i = threadIdx.x; i < kFewRows / split * (D / 4); i += kFewThreads) {
+    const int at = i / (D / 4), r = at * split + part, c = i % (D / 4) * 4;
+    if (r >= here) continue;
+    float m = -INFINITY;
+    for (int p = 0; p < split; ++p) m = max_nan(m, sm.in_ml[p * (kFewRows / split) + at].x);
+    float l = 0.f;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < split; ++p) {
+      const int slot = p * (kFewRows / split) + at;
+      const float2 ml = sm.in_ml[slot];
+      const float4 y = *reinterpret_cast<const float4*>(&sm.in[slot][c]);
+      const float x = m == -INFINITY ? 0.f : ex2_approx(ml.x - m);
+      l += x * ml.y;
+      f.x += x * y.x;
+      f.y += x * y.y;
+      f.z += x * y.z;
+      f.w += x * y.w;
+    }
+    finish(r, c, m, l, f);
+  }
+}
+
+// Blocks of the few-row form that run at once: its registers leave room for one an SM at 128 values a head, two at 64
+int64_t few_slots(int d) { return static_cast<int64_t>(device_sm_count()) * (d == 64 ? 2 : 1); }
+
+// Blocks that share a tile's keys: more while all of them still run at once and every warp keeps 16 keys
+int few_split(int64_t units, int seq_k, int d) {
+  int split = 1;
+  while (split < 8 && 2 * units * split <= few_slots(d) && split * kFewWarps * 16 < seq_k) split *= 2;
+  return split;
 }
 
 template <typename T, int D>
 void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
-  const int64_t tiles = (static_cast<int64_t>(a.seq_q) * (a.heads / a.heads_kv) + 15) / 16;
+  auto kern = cross_few_kernel<T, D>;
+  constexpr int kSmem = sizeof(FewSmem<D>);
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, kSmem, allowed);
+  const int64_t tiles = (static_cast<int64_t>(a.seq_q) * (a.heads / a.heads_kv) + kFewRows - 1) / kFewRows;
   const int64_t units = tiles * a.heads_kv * a.batch;
-  // split the keys while the blocks do not fill the SMs twice and every warp keeps 16 keys
-  int split = 1;
-  while (split < 8 && units * split < 2 * 148 && split * kFewWarps * 16 < a.seq_k) split *= 2;
+  const int split = few_split(units, a.seq_k, D);
   if (tiles * split > 0x7fffffff) throw std::runtime_error("cross_attention: too many queries");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), a.heads_kv, a.batch);
-  cfg.blockDim = dim3(32 * kFewWarps);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -246,7 +290,7 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, cross_few_kernel<T, D>, a, split);
+  cudaLaunchKernelEx(&cfg, kern, a, split);
 }
 
 // ---------------------------------------------------------------------------
@@ -260,7 +304,12 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 // TMEM: S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B [384, 384 + D).  P is written over the first
 // half of its S as the second product's TMEM operand, in two chunks of 64 keys.  O is rescaled only when the
 // running maximum has grown by more than 2^8; P then is at most 256 and exact sums hold in fp32.
-// Bound by the chain softmax, PV, next S of a tile; LATER.
+// Bound by the chain softmax (2000 cycles a step), P to PV, PV, next S (1400) of a tile, which two tiles in turn cover to
+// about 60 % of the tensor pipe's time, and at a unit's end by its output (2500).  32760 queries of 12 heads over 4096
+// keys take 690 us (1190 TFLOP/s), 2 x 32760 over 512 keys 205 us (1000).  Measured and not kept: P through shared memory
+// with the next scores formed during the exponentials (268 us against 240 at 4096 x 4096: operands, P and loads together
+// exceed the shared memory's rate), two threads a row (213 against 197), output warps of their own, every fourth pair of
+// exponentials as a polynomial (238 against 197), a product warp a tile (218 against 197).
 constexpr int kQT = 128, kKT = 128, kPChunks = 2;
 constexpr int kTileThreads = 384;
 
@@ -754,9 +803,28 @@ void launch_tiles(const CrossAttnArgs& a, cudaStream_t s) {
   kern<<<units < sms ? sh.units : sms, kTileThreads, Cfg::kSmemBytes, s>>>(maps, a, sh);
 }
 
+// The form that takes less time, by what both were measured to take in us (in a graph, 1 to 5 batch entries, 4 to 24
+// heads of 64 and 128, 1 to 300 queries, 64 to 4096 keys):
+//   few rows   1.5 (3 with split keys) + waves * (2 + passes over 128 keys)
+//   tiles      3.2 + rounds of units * (1.2 + 1.65 a key tile)
+// e.g. 64 queries of 2 x 12 heads over 1024 keys 12.2 and 17.9, 300 queries of 4 heads over 300 keys 7.6 and 11.2, 128
+// queries of 2 x 12 heads over 300 keys 13.2 and 10.1.
+bool few_is_faster(const CrossAttnArgs& a) {
+  const int group = a.heads / a.heads_kv;
+  const int64_t heads = static_cast<int64_t>(a.heads_kv) * a.batch;
+  const int64_t few = (static_cast<int64_t>(a.seq_q) * group + kFewRows - 1) / kFewRows * heads;
+  const int split = few_split(few, a.seq_k, a.head_dim);
+  const int64_t slots = few_slots(a.head_dim), sms = device_sm_count();
+  const double waves = static_cast<double>((few * split + slots - 1) / slots);
+  const double passes = (a.seq_k + split * kFewWarps * 16 - 1) / (split * kFewWarps * 16);
+  const int64_t units = ((static_cast<int64_t>(a.seq_q) + kQT - 1) / kQT * group + 1) / 2 * heads;
+  const double rounds = static_cast<double>((units + sms - 1) / sms);
+  return (split > 1 ? 3.0 : 1.5) + waves * (2.0 + passes) < 3.2 + rounds * (1.2 + 1.65 * ((a.seq_k + kKT - 1) / kKT));
+}
+
 template <typename T, int D>
 void launch_dim(const CrossAttnArgs& a, cudaStream_t s) {
-  if (static_cast<int64_t>(a.seq_q) * (a.heads / a.heads_kv) <= 64) launch_few<T, D>(a, s);
+  if (few_is_faster(a)) launch_few<T, D>(a, s);
   else launch_tiles<T, D>(a, s);
 }
 
