@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+        if constexpr (kPair) mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[acc]), 0));
         else mbar_arrive(&acc_empty[acc]);
       }
     };
