@@ -4,7 +4,12 @@
 // host's time is what a user waits for.  A call whose arguments are not laid out as its kernel takes them,
 // or are wrong, launches nothing and returns None; ops/ then either brings them into that layout and calls
 // again, or says what is wrong.  What keeps a launch inside its buffers is checked here alone.
+//
+// The entries are plain C functions over the argument vector: converting eight tensor arguments through
+// the binding library took 1.5 us, a quarter of a small call.
 #include <torch/extension.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
@@ -18,7 +23,82 @@
 namespace {
 
 namespace py = pybind11;
-using OptTensor = c10::optional<at::Tensor>;
+
+// An optional tensor argument: a borrowed tensor, or nothing for None
+struct OptTensor {
+  const at::Tensor* t = nullptr;
+  bool has_value() const { return t != nullptr; }
+  const at::Tensor& operator*() const { return *t; }
+  const at::Tensor* operator->() const { return t; }
+};
+
+struct BadArgument : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+const at::Tensor& tensor_arg(PyObject* o) {
+  if (!THPVariable_Check(o)) throw BadArgument(std::string("expected a tensor, got ") + Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+OptTensor opt_arg(PyObject* o) { return o == Py_None ? OptTensor{} : OptTensor{&tensor_arg(o)}; }
+int64_t int_arg(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+double float_arg(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+bool bool_arg(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw py::error_already_set();
+  return v != 0;
+}
+
+PyObject* nothing() { Py_RETURN_NONE; }
+PyObject* wrap(at::Tensor t) {
+  PyObject* o = THPVariable_Wrap(std::move(t));
+  if (o == nullptr) throw py::error_already_set();
+  return o;
+}
+// a new tuple of its arguments' references (nullptr: None)
+PyObject* tuple_of(std::initializer_list<PyObject*> items) {
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(items.size()));
+  Py_ssize_t i = 0;
+  for (PyObject* o : items) {
+    if (o == nullptr) {
+      o = Py_None;
+      Py_INCREF(o);
+    }
+    if (t != nullptr) PyTuple_SET_ITEM(t, i++, o);
+    else Py_DECREF(o);
+  }
+  if (t == nullptr) throw py::error_already_set();
+  return t;
+}
+
+// An entry: a function over `kCount` arguments whose C++ exceptions become Python's
+template <PyObject* (*kBody)(PyObject* const*), int kCount>
+PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != kCount) {
+    PyErr_Format(PyExc_TypeError, "expected %d arguments, got %zd", kCount, n);
+    return nullptr;
+  }
+  try {
+    return kBody(args);
+  } catch (py::error_already_set& e) {
+    e.restore();
+  } catch (const BadArgument& e) {
+    PyErr_SetString(PyExc_TypeError, e.what());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown error");
+  }
+  return nullptr;
+}
 
 // The device status words that ops/_ext.py made, by device index.
 std::mutex status_mu;
@@ -84,7 +164,7 @@ bool is_vector(const at::Tensor& t, const at::Device& dev, int64_t n, at::Scalar
 // whether `out` (rows o) shares no byte with `in` (rows i): other storages, spans that do not meet, or other
 // columns of one buffer
 bool apart(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Rows& i) {
-  if (out.storage().data() != in.storage().data() || o.rows == 0 || i.rows == 0) return true;
+  if (!out.is_alias_of(in) || o.rows == 0 || i.rows == 0) return true;
   const int64_t eo = out.element_size(), ei = in.element_size();
   const int64_t lo = reinterpret_cast<int64_t>(out.data_ptr()), at = reinterpret_cast<int64_t>(in.data_ptr());
   const int64_t hi = lo + ((o.rows - 1) * o.stride + o.cols) * eo, end = at + ((i.rows - 1) * i.stride + i.cols) * ei;
@@ -127,34 +207,38 @@ at::Tensor empty_fp8_like(const at::Tensor& x, const Rows& r) {
   return at::as_strided(buf, x.sizes(), strides);
 }
 
-py::object rms_norm_quant(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps,
-                          const OptTensor& out, const OptTensor& scale_out, const OptTensor& residual_out) {
+// (x, weight, residual, eps, out, scale_out, residual_out) -> (q, scale, h)
+PyObject* rms_norm_quant(PyObject* const* args) {
+  const at::Tensor& x = tensor_arg(args[0]);
+  const OptTensor weight = opt_arg(args[1]), residual = opt_arg(args[2]);
+  const double eps = float_arg(args[3]);
+  const OptTensor out = opt_arg(args[4]), scale_out = opt_arg(args[5]), residual_out = opt_arg(args[6]);
   const at::Device dev = x.device();
   ds::NormQuantArgs a;
   a.type = elem_type(x);
   Rows rx, rr, rh, rq;
-  if (!x.is_cuda() || a.type < 0 || !as_rows(x, dev, rx)) return py::none();
+  if (!x.is_cuda() || a.type < 0 || !as_rows(x, dev, rx)) return nothing();
   if (weight.has_value()) {
-    if (!is_vector(*weight, dev, rx.cols, x.scalar_type())) return py::none();
+    if (!is_vector(*weight, dev, rx.cols, x.scalar_type())) return nothing();
     a.weight = weight->data_ptr();
   }
-  if (residual_out.has_value() && !residual.has_value()) return py::none();
+  if (residual_out.has_value() && !residual.has_value()) return nothing();
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor h;
   if (residual.has_value()) {
     if (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type() || !as_rows(*residual, dev, rr))
-      return py::none();
+      return nothing();
     if (residual_out.has_value()) {
       h = *residual_out;
-      if (h.sizes() != x.sizes() || h.scalar_type() != x.scalar_type() || !as_output(h, dev, rh)) return py::none();
-      if (!apart_or_same(h, rh, x, rx) || !apart_or_same(h, rh, *residual, rr)) return py::none();
+      if (h.sizes() != x.sizes() || h.scalar_type() != x.scalar_type() || !as_output(h, dev, rh)) return nothing();
+      if (!apart_or_same(h, rh, x, rx) || !apart_or_same(h, rh, *residual, rr)) return nothing();
     }
   }
   if (out.has_value() && (out->sizes() != x.sizes() || out->scalar_type() != at::kFloat8_e4m3fn || !as_output(*out, dev, rq)))
-    return py::none();
+    return nothing();
   if (scale_out.has_value() && (scale_out->sizes() != x.sizes().slice(0, x.dim() - 1) || !scale_out->is_contiguous() ||
                                 scale_out->scalar_type() != at::kFloat || scale_out->device() != dev))
-    return py::none();
+    return nothing();
   if (residual.has_value()) {
     if (!residual_out.has_value()) {
       h = empty(x.sizes(), x.scalar_type(), dev);
@@ -178,7 +262,7 @@ py::object rms_norm_quant(const at::Tensor& x, const OptTensor& weight, const Op
   a.eps = static_cast<float>(eps);
   ds::launch_norm_quant(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return py::make_tuple(std::move(q), std::move(scale), residual.has_value() ? py::cast(std::move(h)) : py::none());
+  return tuple_of({wrap(std::move(q)), wrap(std::move(scale)), residual.has_value() ? wrap(std::move(h)) : nullptr});
 }
 
 // e4m3 rows that the product's 16-byte loads and tile loads can take
@@ -189,41 +273,47 @@ bool fp8_rows(const at::Tensor& t, const at::Device& dev, Rows& r) {
   return r.stride % 16 == 0 && r.stride >= r.cols;
 }
 
-py::object linear_fp8(const at::Tensor& x, const at::Tensor& sx, const at::Tensor& w, const at::Tensor& sw,
-                      const OptTensor& bias, bool gelu, const OptTensor& residual, const OptTensor& gate,
-                      c10::optional<int64_t> rows_per_batch, const OptTensor& row_batch, const OptTensor& out,
-                      at::ScalarType out_type) {
-  if (!x.is_cuda()) return py::none();
+// (x, x_scale, w, w_scale, bias, gelu, residual, gate, rows_per_batch, row_batch, out, out_dtype) -> y
+PyObject* linear_fp8(PyObject* const* args) {
+  const at::Tensor &x = tensor_arg(args[0]), &sx = tensor_arg(args[1]), &w = tensor_arg(args[2]), &sw = tensor_arg(args[3]);
+  const OptTensor bias = opt_arg(args[4]);
+  const bool gelu = bool_arg(args[5]);
+  const OptTensor residual = opt_arg(args[6]), gate = opt_arg(args[7]);
+  const int64_t rows_per_batch = args[8] == Py_None ? 0 : int_arg(args[8]);  // 0: not given
+  const OptTensor row_batch = opt_arg(args[9]), out = opt_arg(args[10]);
+  if (!THPDtype_Check(args[11])) throw BadArgument("out_dtype must be a dtype");
+  at::ScalarType out_type = reinterpret_cast<THPDtype*>(args[11])->scalar_type;
+  if (!x.is_cuda()) return nothing();
   const at::Device dev = x.device();
   Rows rx, rw, ry, rr;
   ds::LinearFp8Args a;
   a.status = status_of(dev);
   if (a.status == nullptr || !fp8_rows(x, dev, rx) || w.dim() != 2 || !fp8_rows(w, dev, rw) || rw.cols != rx.cols)
-    return py::none();
+    return nothing();
   const int64_t M = rx.rows, K = rx.cols, N = rw.rows;
-  if (M > (1 << 30) || N > (1 << 30)) return py::none();
+  if (M > (1 << 30) || N > (1 << 30)) return nothing();
   if (sx.sizes() != x.sizes().slice(0, x.dim() - 1) || sx.scalar_type() != at::kFloat || sx.device() != dev ||
       !sx.is_contiguous() || !is_vector(sw, dev, N, at::kFloat))
-    return py::none();
-  if (gelu && residual.has_value()) return py::none();
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    return nothing();
+  if (gelu && residual.has_value()) return nothing();
+  at::DimVector shape(x.sizes());
   shape.back() = N;
   if (out.has_value()) {
     out_type = out->scalar_type();
-    if (out->sizes() != at::IntArrayRef(shape) || (N > 0 && !as_output(*out, dev, ry))) return py::none();
+    if (out->sizes() != at::IntArrayRef(shape) || (N > 0 && !as_output(*out, dev, ry))) return nothing();
   } else {
     ry.stride = N;
   }
-  if (out_type != at::kBFloat16 && out_type != at::kHalf && out_type != at::kFloat) return py::none();
+  if (out_type != at::kBFloat16 && out_type != at::kHalf && out_type != at::kFloat) return nothing();
   if (bias.has_value()) {
-    if (!is_vector(*bias, dev, N, out_type)) return py::none();
+    if (!is_vector(*bias, dev, N, out_type)) return nothing();
     a.bias = bias->data_ptr();
   }
   if (residual.has_value()) {
     if (residual->sizes() != at::IntArrayRef(shape) || residual->scalar_type() != out_type ||
         (N > 0 && !as_rows(*residual, dev, rr)))
-      return py::none();
-    if (out.has_value() && N > 0 && !apart_or_same(*out, ry, *residual, rr)) return py::none();
+      return nothing();
+    if (out.has_value() && N > 0 && !apart_or_same(*out, ry, *residual, rr)) return nothing();
     a.residual = residual->data_ptr();
     a.ldr = rr.stride;
   }
@@ -231,19 +321,19 @@ py::object linear_fp8(const at::Tensor& x, const at::Tensor& sx, const at::Tenso
     const at::Tensor& g = *gate;
     if (!residual.has_value() || g.scalar_type() != at::kFloat || g.device() != dev || g.dim() < 1 || g.dim() > 2 ||
         g.size(-1) != N || (N > 1 && g.stride(-1) != 1))
-      return py::none();
+      return nothing();
     const int64_t batches = g.dim() == 2 ? g.size(0) : 1;
-    const int64_t per = rows_per_batch.has_value() ? *rows_per_batch : std::max<int64_t>(M, 1);
-    if (batches < 1 || per < 1) return py::none();
+    const int64_t per = args[8] != Py_None ? rows_per_batch : std::max<int64_t>(M, 1);
+    if (batches < 1 || per < 1) return nothing();
     a.gate = g.data_ptr<float>();
     a.gate_stride = g.dim() == 2 ? g.stride(0) : 0;
     a.batches = static_cast<int>(std::min<int64_t>(batches, 1 << 30));
     a.rows_per_batch = static_cast<int>(std::min<int64_t>(per, 1 << 30));
     if (row_batch.has_value()) {
-      if (!is_vector(*row_batch, dev, M, at::kInt)) return py::none();
+      if (!is_vector(*row_batch, dev, M, at::kInt)) return nothing();
       a.row_batch = row_batch->data_ptr<int>();
     } else if ((M + per - 1) / per > batches) {
-      return py::none();
+      return nothing();
     }
   }
   const c10::cuda::CUDAGuard guard(dev);
@@ -263,7 +353,7 @@ py::object linear_fp8(const at::Tensor& x, const at::Tensor& sx, const at::Tenso
   a.gelu = gelu ? 1 : 0;
   ds::launch_linear_fp8(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return py::cast(std::move(y));
+  return wrap(std::move(y));
 }
 
 // What a rotation's axes and thetas fix: the axis and frequency of every pair.
@@ -293,35 +383,42 @@ py::object rope_plan(const std::vector<int64_t>& dims, const std::vector<double>
   return py::cast(p);
 }
 
-py::object rope_axes(const at::Tensor& x, const OptTensor& k, const at::Tensor& pos, const RopePlan& plan,
-                     int64_t head_dim, bool half, bool inverse, const OptTensor& out, const OptTensor& k_out) {
-  if (!x.is_cuda()) return py::none();
+// (x, k, positions, plan, head_dim, half, inverse, out, k_out) -> x' or (x', k')
+PyObject* rope_axes(PyObject* const* args) {
+  const at::Tensor& x = tensor_arg(args[0]);
+  const OptTensor k = opt_arg(args[1]);
+  const at::Tensor& pos = tensor_arg(args[2]);
+  const RopePlan& plan = py::handle(args[3]).cast<const RopePlan&>();
+  const int64_t head_dim = int_arg(args[4]);
+  const bool half = bool_arg(args[5]), inverse = bool_arg(args[6]);
+  const OptTensor out = opt_arg(args[7]), k_out = opt_arg(args[8]);
+  if (!x.is_cuda()) return nothing();
   const at::Device dev = x.device();
   ds::RopeAxesArgs a;
   a.type = elem_type(x);
   if (a.type < 0 || head_dim < 2 * plan.pairs || head_dim > (1 << 20) || (k_out.has_value() && !k.has_value()))
-    return py::none();
+    return nothing();
   const int64_t pos_axes = pos.dim() == 1 ? 1 : (pos.dim() == 2 ? pos.size(1) : 0);
-  if (pos.device() != dev || pos_axes != plan.axes) return py::none();
+  if (pos.device() != dev || pos_axes != plan.axes) return nothing();
   switch (pos.scalar_type()) {
     case at::kLong: a.pos_type = 0; break;
     case at::kInt: a.pos_type = 1; break;
     case at::kFloat: a.pos_type = 2; break;
     case at::kDouble: a.pos_type = 3; break;
-    default: return py::none();
+    default: return nothing();
   }
   Rows in[2], to[2];
-  const at::Tensor* t[2] = {&x, k.has_value() ? &*k : nullptr};
-  const OptTensor* o[2] = {&out, &k_out};
+  const at::Tensor* t[2] = {&x, k.t};
+  const OptTensor o[2] = {out, k_out};
   for (int i = 0; i < 2 && t[i] != nullptr; ++i) {
     if (t[i]->dim() < 2 || t[i]->scalar_type() != x.scalar_type() || !as_rows(*t[i], dev, in[i]) ||
         in[i].cols % head_dim != 0 || in[i].rows != in[0].rows)
-      return py::none();
-    if (o[i]->has_value()) {
-      const at::Tensor& y = **o[i];
+      return nothing();
+    if (o[i].has_value()) {
+      const at::Tensor& y = *o[i];
       if (y.sizes() != t[i]->sizes() || y.scalar_type() != x.scalar_type() || !as_output(y, dev, to[i]) ||
           !apart_or_same(y, to[i], *t[i], in[i]))
-        return py::none();
+        return nothing();
     } else {
       to[i].stride = in[i].cols;
     }
@@ -330,13 +427,13 @@ py::object rope_axes(const at::Tensor& x, const OptTensor& k, const at::Tensor& 
   if (k.has_value() && ((out.has_value() && !apart(*out, to[0], *k, in[1])) ||
                         (k_out.has_value() && !apart(*k_out, to[1], x, in[0])) ||
                         (out.has_value() && k_out.has_value() && !apart(*out, to[0], *k_out, to[1]))))
-    return py::none();
+    return nothing();
   const int64_t rows = in[0].rows;
-  if (rows > 0 && (pos.size(0) == 0 || rows % pos.size(0) != 0)) return py::none();
+  if (rows > 0 && (pos.size(0) == 0 || rows % pos.size(0) != 0)) return nothing();
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor y[2];
   for (int i = 0; i < 2 && t[i] != nullptr; ++i) {
-    y[i] = o[i]->has_value() ? **o[i] : empty(t[i]->sizes(), x.scalar_type(), dev);
+    y[i] = o[i].has_value() ? *o[i] : empty(t[i]->sizes(), x.scalar_type(), dev);
     a.t[i].x = t[i]->data_ptr();
     a.t[i].x_stride = in[i].stride;
     a.t[i].y = y[i].data_ptr();
@@ -356,24 +453,27 @@ py::object rope_axes(const at::Tensor& x, const OptTensor& k, const at::Tensor& 
   std::copy(plan.axis, plan.axis + plan.pairs, a.axis);
   ds::launch_rope_axes(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (t[1] == nullptr) return py::cast(std::move(y[0]));
-  return py::make_tuple(std::move(y[0]), std::move(y[1]));
+  if (t[1] == nullptr) return wrap(std::move(y[0]));
+  return tuple_of({wrap(std::move(y[0])), wrap(std::move(y[1]))});
 }
 
-py::object cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t heads, int64_t heads_kv,
-                           const OptTensor& kv_lens, const OptTensor& key_mask, c10::optional<double> scale,
-                           const OptTensor& out, bool return_lse) {
-  if (!q.is_cuda() || q.dim() != 3 || k.dim() != 3 || heads < 1 || heads_kv < 1 || heads % heads_kv != 0) return py::none();
+// (q, k, v, heads, heads_kv, kv_lens, key_mask, scale, out, return_lse) -> out or (out, lse)
+PyObject* cross_attention(PyObject* const* args) {
+  const at::Tensor &q = tensor_arg(args[0]), &k = tensor_arg(args[1]), &v = tensor_arg(args[2]);
+  const int64_t heads = int_arg(args[3]), heads_kv = int_arg(args[4]);
+  const OptTensor kv_lens = opt_arg(args[5]), key_mask = opt_arg(args[6]), out = opt_arg(args[8]);
+  const bool return_lse = bool_arg(args[9]);
+  if (!q.is_cuda() || q.dim() != 3 || k.dim() != 3 || heads < 1 || heads_kv < 1 || heads % heads_kv != 0) return nothing();
   const at::Device dev = q.device();
   ds::CrossAttnArgs a;
   a.type = elem_type(q);
   a.status = status_of(dev);
   const int64_t B = q.size(0), Sq = q.size(1), width = q.size(2), Sk = k.size(1), d = width / heads;
   if (a.status == nullptr || (a.type != ds::kBF16 && a.type != ds::kFP16) || width % heads != 0 || (d != 64 && d != 128))
-    return py::none();
+    return nothing();
   if (B < 1 || B > 65535 || heads_kv > 65535 || Sq < 1 || Sk < 1 || Sk >= (int64_t{1} << 30) ||
       Sq * (heads / heads_kv) >= (int64_t{1} << 30) || width >= (int64_t{1} << 30))
-    return py::none();
+    return nothing();
   auto fits = [&](const at::Tensor& t, int64_t rows, int64_t cols, bool output) {
     if (t.device() != dev || t.scalar_type() != q.scalar_type() || t.dim() != 3 || t.size(0) != B || t.size(1) != rows ||
         t.size(2) != cols || t.stride(2) != 1 || t.stride(1) % 8 != 0 || t.stride(0) % 8 != 0 ||
@@ -382,26 +482,26 @@ py::object cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (rows > 1 && t.stride(1) < (output ? cols : 8)) return false;
     return !output || B == 1 || t.stride(0) >= cols;
   };
-  if (!fits(q, Sq, width, false) || !fits(k, Sk, heads_kv * d, false) || !fits(v, Sk, heads_kv * d, false)) return py::none();
+  if (!fits(q, Sq, width, false) || !fits(k, Sk, heads_kv * d, false) || !fits(v, Sk, heads_kv * d, false)) return nothing();
   if (out.has_value()) {
-    if (!fits(*out, Sq, width, true)) return py::none();
+    if (!fits(*out, Sq, width, true)) return nothing();
     for (const at::Tensor* t : {&q, &k, &v})
-      if (spans_meet(*out, *t)) return py::none();
+      if (spans_meet(*out, *t)) return nothing();
   }
   if (kv_lens.has_value()) {
-    if (!is_vector(*kv_lens, dev, B, at::kInt)) return py::none();
+    if (!is_vector(*kv_lens, dev, B, at::kInt)) return nothing();
     a.kv_lens = kv_lens->data_ptr<int>();
   }
   if (key_mask.has_value()) {
     const at::Tensor& m = *key_mask;
     if (m.device() != dev || m.scalar_type() != at::kBool || m.dim() != 2 || m.size(0) != B || m.size(1) != Sk)
-      return py::none();
+      return nothing();
     a.key_mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
     a.mask_row = m.stride(0);
     a.mask_col = m.stride(1);
   }
-  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(d));
-  if (!(s > 0.0) || !std::isfinite(s)) return py::none();
+  const double s = args[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : float_arg(args[7]);
+  if (!(s > 0.0) || !std::isfinite(s)) return nothing();
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor o = out.has_value() ? *out : empty(q.sizes(), q.scalar_type(), dev), lse;
   if (return_lse) {
@@ -425,18 +525,25 @@ py::object cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   a.scale = static_cast<float>(s);
   ds::launch_cross_attention(a, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (!return_lse) return py::cast(std::move(o));
-  return py::make_tuple(std::move(o), std::move(lse));
+  if (!return_lse) return wrap(std::move(o));
+  return tuple_of({wrap(std::move(o)), wrap(std::move(lse))});
+}
+
+template <PyObject* (*kBody)(PyObject* const*), int kCount>
+void add_entry(pybind11::module_& m, const char* name, const char* doc) {
+  static PyMethodDef def = {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<kBody, kCount>)),
+                            METH_FASTCALL, doc};
+  m.add_object(name, py::reinterpret_steal<py::object>(PyCFunction_New(&def, nullptr)));
 }
 
 }  // namespace
 
 void bind_block_ops(pybind11::module_& m) {
   m.def("bind_status", &bind_status, "names a device's status word to the block operators");
-  m.def("rms_norm_quant", &rms_norm_quant, "residual addition + RMS norm + e4m3 rows with scales");
-  m.def("linear_fp8", &linear_fp8, "linear layer on e4m3 operands with row scales");
   py::class_<RopePlan>(m, "RopePlan");
   m.def("rope_plan", &rope_plan, "the frequencies of a set of axes, or None");
-  m.def("rope_axes", &rope_axes, "rotary positions with several axes");
-  m.def("cross_attention", &cross_attention, "attention to padded, masked encoder states");
+  add_entry<&rms_norm_quant, 7>(m, "rms_norm_quant", "residual addition + RMS norm + e4m3 rows with scales");
+  add_entry<&linear_fp8, 12>(m, "linear_fp8", "linear layer on e4m3 operands with row scales");
+  add_entry<&rope_axes, 9>(m, "rope_axes", "rotary positions with several axes");
+  add_entry<&cross_attention, 10>(m, "cross_attention", "attention to padded, masked encoder states");
 }
