@@ -3,6 +3,8 @@
 //   y[m, n] = epilogue(sx[m] * sw[n] * sum_k x[m, k] * w[n, k] + b[n])
 //
 // x and w are e4m3 with one fp32 scale a row (a token, an output channel); sums are fp32.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "elem.cuh"
@@ -13,6 +15,8 @@
 
 namespace ds {
 namespace {
+
+namespace cg = cooperative_groups;
 
 // bias, activation, gate and residual of one output value; v is the scaled sum
 template <typename T>
@@ -45,53 +49,128 @@ __device__ __forceinline__ const float* gate_of(const LinearFp8Args& a, int m) {
 __device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
   if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t w[4] = {0, 0, 0, 0};
+  if (k >= K) return make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     if (k + i < K) w[i >> 2] |= static_cast<uint32_t>(row[k + i]) << (8 * (i & 3));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Few rows: a block takes 16 output channels and 8 * kM rows of x; its warps split K in chunks of 64
-// and join their sums in shared memory.  The weights are the product's A operand straight from
-// global memory, read once: bound by HBM.
+// Few rows: a block takes 16 output channels and 8 * kM rows of x; its warps split K in chunks of 64, and so do up
+// to 8 blocks of a cluster where channels are few and K is long.  The weights are the product's A operand
+// straight from global memory, read once; sums are joined in shared memory, in a fixed order.  Bound by HBM, for
+// small weights by latency: 2 rows to 9216 channels from 1536 values take 4.7 us on the device, 1 row to 256 channels
+// from 8192 values 3.5 (7.5 with K in one block's warps alone).
 constexpr int kRowWarps = 8;
 
+template <int kM>
+struct RowSmem {
+  float part[kRowWarps][kM * 8][17];
+  float in[8][kM * 8][16];  // rank 0: the cluster's sums
+};
+
 template <typename T, int kM>
-__global__ void __launch_bounds__(32 * kRowWarps) linear_rows_kernel(LinearFp8Args a) {
-  __shared__ float part[kRowWarps][kM * 8][17];
+__global__ void __launch_bounds__(32 * kRowWarps) linear_rows_kernel(LinearFp8Args a, int split) {
+  extern __shared__ __align__(16) uint8_t row_smem[];
+  RowSmem<kM>& sm = *reinterpret_cast<RowSmem<kM>*>(row_smem);
+  cg::cluster_group cluster = cg::this_cluster();
+  if (split > 1) cluster.barrier_arrive();  // waited for below: no push before all blocks have started
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (8 * kM);
-  // rows behind the last are read as the last one and their sums dropped
-  const uint8_t* w0 = a.w + static_cast<int64_t>(min(n0 + g, a.N - 1)) * a.ldw;
-  const uint8_t* w1 = a.w + static_cast<int64_t>(min(n0 + g + 8, a.N - 1)) * a.ldw;
-  float acc[kM][4] = {};
-  for (int k = warp * 64 + t * 16; k - t * 16 < a.K; k += 64 * kRowWarps) {
-    const uint4 u = load16(w0, k, a.K), v = load16(w1, k, a.K);
+  const int rank = blockIdx.x % split;  // the cluster's blocks are neighbours in x
+  const int n0 = blockIdx.x / split * 16, m0 = blockIdx.y * (8 * kM);
+  // channels and rows behind the last are read as the last one and their sums dropped
+  const uint8_t* w[2];
 #pragma unroll
-    for (int i = 0; i < kM; ++i) {
-      const int m = min(m0 + i * 8 + g, a.M - 1);
-      const uint4 b = load16(a.x + static_cast<int64_t>(m) * a.ldx, k, a.K);
-      mma16832_e4m3(acc[i], u.x, v.x, u.y, v.y, b.x, b.y);
-      mma16832_e4m3(acc[i], u.z, v.z, u.w, v.w, b.z, b.w);
+  for (int i = 0; i < 2; ++i) w[i] = a.w + static_cast<int64_t>(min(n0 + i * 8 + g, a.N - 1)) * a.ldw;
+  const uint8_t* x[kM];
+#pragma unroll
+  for (int i = 0; i < kM; ++i) x[i] = a.x + static_cast<int64_t>(min(m0 + i * 8 + g, a.M - 1)) * a.ldx;
+  float acc[kM][4] = {};
+  const int step = 64 * kRowWarps * split;
+  for (int k0 = (rank * kRowWarps + warp) * 64; k0 < a.K; k0 += 2 * step) {
+    uint4 wf[2][2], xf[2][kM];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // the loads of two chunks before the products of the first
+      const int k = k0 + u * step + t * 16;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) wf[u][i] = load16(w[i], k, a.K);
+#pragma unroll
+      for (int i = 0; i < kM; ++i) xf[u][i] = load16(x[i], k, a.K);
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < kM; ++i) {
+        const uint4 p = wf[u][0], q = wf[u][1], b = xf[u][i];
+        mma16832_e4m3(acc[i], p.x, q.x, p.y, q.y, b.x, b.y);
+        mma16832_e4m3(acc[i], p.z, q.z, p.w, q.w, b.z, b.w);
+      }
   }
 #pragma unroll
   for (int i = 0; i < kM; ++i) {
-    part[warp][i * 8 + 2 * t][g] = acc[i][0];
-    part[warp][i * 8 + 2 * t + 1][g] = acc[i][1];
-    part[warp][i * 8 + 2 * t][g + 8] = acc[i][2];
-    part[warp][i * 8 + 2 * t + 1][g + 8] = acc[i][3];
+    sm.part[warp][i * 8 + 2 * t][g] = acc[i][0];
+    sm.part[warp][i * 8 + 2 * t + 1][g] = acc[i][1];
+    sm.part[warp][i * 8 + 2 * t][g + 8] = acc[i][2];
+    sm.part[warp][i * 8 + 2 * t + 1][g + 8] = acc[i][3];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kM * 8 * 16; i += 32 * kRowWarps) {
-    const int m = m0 + i / 16, n = n0 + i % 16;
-    if (m >= a.M || n >= a.N) continue;
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) v += part[w][i / 16][i % 16];
+  if (split > 1) cluster.barrier_wait();
+  const int rows = min(8 * kM, a.M - m0);
+  auto store = [&](int r, int c, float v) {
+    const int m = m0 + r, n = n0 + c;
     v *= a.sx[m * a.sx_stride] * a.sw[n * a.sw_stride];
     reinterpret_cast<T*>(a.y)[static_cast<int64_t>(m) * a.ldy + n] = from_float<T>(finish<T>(a, v, m, n, gate_of(a, m)));
+  };
+  RowSmem<kM>* to = split > 1 ? cluster.map_shared_rank(&sm, 0) : &sm;
+  for (int i = threadIdx.x; i < rows * 16; i += 32 * kRowWarps) {
+    const int r = i / 16, c = i % 16;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < kRowWarps; ++q) v += sm.part[q][r][c];
+    if (split > 1) to->in[rank][r][c] = v;
+    else if (n0 + c < a.N) store(r, c, v);
   }
+  if (split == 1) return;
+  cluster.sync();
+  if (rank != 0) return;
+  for (int i = threadIdx.x; i < rows * 16; i += 32 * kRowWarps) {
+    const int r = i / 16, c = i % 16;
+    if (n0 + c >= a.N) continue;
+    float v = 0.f;
+    for (int p = 0; p < split; ++p) v += sm.in[p][r][c];
+    store(r, c, v);
+  }
+}
+
+// Blocks that share K: more while the blocks leave SMs without one and every warp keeps two chunks
+int row_split(int64_t blocks, int K) {
+  int split = 1;
+  while (split < 8 && 2 * blocks * split <= device_sm_count() && 2 * split * kRowWarps * 128 <= K) split *= 2;
+  return split;
+}
+
+template <typename T, int kM>
+void launch_rows(const LinearFp8Args& a, cudaStream_t s) {
+  auto kern = linear_rows_kernel<T, kM>;
+  constexpr int kSmem = sizeof(RowSmem<kM>);
+  static std::atomic<uint64_t> allowed{0};
+  if (kSmem > 48 * 1024) allow_smem(kern, kSmem, allowed);
+  const int64_t gx = (static_cast<int64_t>(a.N) + 15) / 16, gy = (a.M + 8 * kM - 1) / (8 * kM);
+  const int split = row_split(gx * gy, a.K);
+  if (gx * split > 0x7fffffff) throw std::runtime_error("linear_fp8: too many channels");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(gx * split), static_cast<unsigned>(gy));
+  cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, a, split);
 }
 
 // ---------------------------------------------------------------------------
@@ -399,7 +478,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tma_store_commit();
           }
         } else if (row_ok) {
-          // rows off 16 bytes, and the 16 columns that a tile of odd width leaves behind its last unit
+          // rows off 16 bytes
           const int end = min(min(kU, sh.bn - c), a.N - n);
           T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
 #pragma unroll
@@ -471,14 +550,16 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, a, sh);
 }
 
-// Width of the tiles: the multiple of 16 whose rounds over the SMs cost least.  A k-block takes about 0.29 us +
+// Width of the tiles: the multiple of a unit whose rounds over the SMs cost least.  A k-block takes about 0.29 us +
 // 0.1 us * bn / 256 (8960 x 1536 channels at 32760 rows: 0.39, 0.355 and 0.325 us for 256, 192 and 128
 // channels), bound by the L2's traffic into shared memory more than by the products, so few wide rounds
 // beat many narrow ones, and a single round takes the narrowest tile that keeps it one.
-int pick_bn(int64_t num_m, int N, int slots) {
+// `unit` (16 or 32) keeps whole 64-byte units of the output in a tile: the columns behind the last whole unit go out one
+// element at a time.
+int pick_bn(int64_t num_m, int N, int slots, int unit) {
   int best = kMaxBn;
   int64_t cost = INT64_MAX;
-  for (int bn = kMaxBn; bn >= 32; bn -= 16) {
+  for (int bn = kMaxBn; bn >= 32; bn -= unit) {
     const int64_t tiles = num_m * ((N + bn - 1) / bn);
     const int64_t c = (tiles + slots - 1) / slots * (bn + 740);
     if (c < cost) {
@@ -489,19 +570,35 @@ int pick_bn(int64_t num_m, int N, int slots) {
   return best;
 }
 
+// Whether the few-row form takes less time, by what both were measured to take in us (in a graph, 12 to 256 rows, 64 to
+// 10240 channels and values; up to 16 rows the first form always):
+//   rows    2 (3.5 with K split over blocks) + the operands' bytes out of L2, 16 + 8 kM rows a block, at 4.8 TB/s
+//   tiles   3.2 + rounds * (k-blocks * (0.24 + 0.1 bn / 256) + 0.6)
+// e.g. 32 rows to 1024 channels from 4096 values 6.4 and 11.3, to 9216 from 1536 10.3 and 8.2.
+bool rows_are_faster(const LinearFp8Args& a) {
+  if (a.M <= 16 || a.M > 4096) return a.M <= 16;
+  const int rows = 32;
+  const int64_t blocks = (static_cast<int64_t>(a.N) + 15) / 16 * ((a.M + rows - 1) / rows);
+  const double few = (row_split(blocks, a.K) > 1 ? 3.5 : 2.0) + static_cast<double>(blocks) * (16 + rows) * a.K / 4.8e6;
+  const int m = a.M <= kBM ? kBM : 2 * kBM, slots = device_sm_count() * kBM / m;
+  const int64_t num_m = (a.M + m - 1) / m;
+  const int bn = pick_bn(num_m, a.N, slots, a.out_type == kFP32 ? 16 : 32);
+  const double rounds = static_cast<double>((num_m * ((a.N + bn - 1) / bn) + slots - 1) / slots);
+  return few < 3.2 + rounds * ((a.K + kBK - 1) / kBK * (0.24 + 0.1 * bn / 256) + 0.6);
+}
+
 template <typename T>
 void launch_type(const LinearFp8Args& a, cudaStream_t s) {
-  const unsigned gx = (a.N + 15) / 16;
   if (a.M <= 8) {
-    linear_rows_kernel<T, 1><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
-  } else if (a.M <= 16) {
-    linear_rows_kernel<T, 2><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
-  } else if (a.M <= 32) {
-    linear_rows_kernel<T, 4><<<dim3(gx, 1), 32 * kRowWarps, 0, s>>>(a);
+    launch_rows<T, 1>(a, s);
+  } else if (rows_are_faster(a)) {
+    if (a.M <= 16) launch_rows<T, 2>(a, s);
+    else launch_rows<T, 4>(a, s);
   } else {
     const int sms = device_sm_count();
-    if (a.M <= kBM) launch_tiles<T, false>(a, pick_bn(1, a.N, sms), s);
-    else launch_tiles<T, true>(a, pick_bn((a.M + 2 * kBM - 1) / (2 * kBM), a.N, sms / 2), s);
+    constexpr int kUnit = 64 / sizeof(T);
+    if (a.M <= kBM) launch_tiles<T, false>(a, pick_bn(1, a.N, sms, kUnit), s);
+    else launch_tiles<T, true>(a, pick_bn((a.M + 2 * kBM - 1) / (2 * kBM), a.N, sms / 2, kUnit), s);
   }
 }
 
