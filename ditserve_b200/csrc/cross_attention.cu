@@ -317,13 +317,16 @@ constexpr int kTileThreads = 384;
 // rows by their threads took 3700 cycles of 18400 a unit of four key tiles
 constexpr int kOutBytes = 32 * 128;
 
+// Batch entries whose keys a block lists, and bytes of mask it reads for that at most
+constexpr int kListed = 64, kListedMask = 1 << 16;
+
 template <int D>
 struct TileCfg {
   static constexpr int kAtoms = D / 64;
   static constexpr int kQBytes = kQT * D * 2;
   static constexpr int kKvBytes = kKT * D * 2;
   static constexpr int kStages = D == 128 ? 2 : 4;  // of K and of V
-  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 8 * kOutBytes + 1024 + 512;
+  static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kKvBytes + 8 * kOutBytes + kListed * 4 + 1024 + 512;
 };
 
 struct TileMaps {
@@ -334,6 +337,7 @@ struct TileShape {
   int units, tiles, group;                  // unit = (b * heads_kv + hk) * pairs + pair of a key head's row tiles
   FastDiv pairs, heads_kv, q_tiles;
   int k_shared, v_shared, q_shared;  // batch stride 0: one entry read by all
+  int listed;                        // the block lists the keys of every batch entry first
 };
 
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
@@ -350,17 +354,20 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 struct Unit {
-  int b, hk, pair, n;  // batch entry, key head, pair of row tiles, key tiles
-  bool two;            // tile B has rows
+  int b, hk, pair;   // batch entry, key head, pair of row tiles
+  int valid, n;      // keys up to the last one that is left, and their tiles
+  bool two;          // tile B has rows
 };
 
-__device__ __forceinline__ Unit unit_of(const CrossAttnArgs& a, const TileShape& sh, int u) {
+// `ends`: the batch entries' keys, where the block has listed them
+__device__ __forceinline__ Unit unit_of(const CrossAttnArgs& a, const TileShape& sh, const int* ends, int u) {
   Unit x;
   const int bh = sh.pairs.div(u);
   x.pair = u - bh * sh.pairs.d;
   x.b = sh.heads_kv.div(bh);
   x.hk = bh - x.b * a.heads_kv;
-  x.n = (valid_keys(a, x.b) + kKT - 1) / kKT;
+  x.valid = sh.listed ? ends[x.b] : valid_keys(a, x.b);
+  x.n = (x.valid + kKT - 1) / kKT;
   x.two = 2 * x.pair + 1 < sh.tiles;
   return x;
 }
@@ -376,19 +383,19 @@ __device__ __forceinline__ int2 tile_of(const CrossAttnArgs& a, const TileShape&
 struct Step {
   int u, j = 0, base = 0;
   Unit x;
-  __device__ __forceinline__ bool settle(const CrossAttnArgs& a, const TileShape& sh) {
+  __device__ __forceinline__ bool settle(const CrossAttnArgs& a, const TileShape& sh, const int* ends) {
     for (; u < sh.units; u += gridDim.x) {
-      x = unit_of(a, sh, u);
+      x = unit_of(a, sh, ends, u);
       if (x.n > 0) return true;
     }
     return false;
   }
-  __device__ __forceinline__ bool advance(const CrossAttnArgs& a, const TileShape& sh) {
+  __device__ __forceinline__ bool advance(const CrossAttnArgs& a, const TileShape& sh, const int* ends) {
     if (++j < x.n) return true;
     j = 0;
     base += x.n;
     u += gridDim.x;
-    return settle(a, sh);
+    return settle(a, sh, ends);
   }
 };
 
@@ -411,7 +418,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* sK = sQ + 2 * Cfg::kQBytes;
   uint8_t* sV = sK + ST * Cfg::kKvBytes;
   uint8_t* sOut = sV + ST * Cfg::kKvBytes;                               // [8 warps]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sOut + 8 * kOutBytes);  // [2] a tile
+  int* ends = reinterpret_cast<int*>(sOut + 8 * kOutBytes);              // [kListed]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ends + kListed);        // [2] a tile
   uint64_t* q_empty = q_full + 2;
   uint64_t* k_full = q_empty + 2;   // [ST]
   uint64_t* k_empty = k_full + ST;
@@ -446,6 +454,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc<512>(tmem_slot);
+  if (sh.listed) {
+    // keys up to the last one that length and mask leave: padding given by a mask alone is left out, too
+    for (int b = warp; b < a.batch; b += kTileThreads / 32) {
+      int end = valid_keys(a, b);
+      if (a.key_mask != nullptr) {
+        int last = 0;
+#pragma unroll 8
+        for (int j = lane; j < end; j += 32)
+          if (a.key_mask[b * a.mask_row + j * a.mask_col] != 0) last = j + 1;
+        end = __reduce_max_sync(0xffffffffu, last);
+      }
+      if (lane == 0) ends[b] = end;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -486,10 +508,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         };
         Step cur;
         cur.u = blockIdx.x;
-        bool ok = cur.settle(a, sh) && load_q(cur.x) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412);
+        bool ok = cur.settle(a, sh, ends) && load_q(cur.x) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412);
         while (ok) {
           Step next = cur;
-          const bool more = next.advance(a, sh);
+          const bool more = next.advance(a, sh, ends);
           // at a unit's end its last V comes before the next unit's Q, which waits for the last scores
           const bool fresh = more && next.j == 0;
           if (fresh && (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413) || !load_q(next.x))) break;
@@ -557,10 +579,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       };
       Step cur;
       cur.u = blockIdx.x;
-      bool ok = cur.settle(a, sh) && issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
+      bool ok = cur.settle(a, sh, ends) && issue_s(0, cur) && (!cur.x.two || issue_s(1, cur));
       while (ok) {
         Step next = cur;
-        const bool more = next.advance(a, sh);
+        const bool more = next.advance(a, sh, ends);
         if (!issue_pv(0, cur) || (more && !issue_s(0, next))) break;
         if (cur.x.two && !issue_pv(1, cur)) break;
         if (more && next.x.two && !issue_s(1, next)) break;
@@ -573,10 +595,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         Step s;
         s.u = blockIdx.x;
         int vc = 0;
-        for (bool ok = s.settle(a, sh); ok; ok = s.advance(a, sh), ++vc) {
+        for (bool ok = s.settle(a, sh, ends); ok; ok = s.advance(a, sh, ends), ++vc) {
           const int st = vc % ST;
           uint32_t w[4];
-          tile_mask(a, s.x.b, s.j, valid_keys(a, s.x.b), w);
+          tile_mask(a, s.x.b, s.j, s.x.valid, w);
           // every lane waits, so that what TMA wrote is ordered before its stores
           if (!mbar_wait_warp(&v_full[st], (vc / ST) & 1, abort_flag, a.status, 430)) break;
   #pragma unroll
@@ -617,9 +639,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     int step = 0;  // key tiles of tile t so far: the phase of its barriers
     bool ok = true;
     for (int u = blockIdx.x; ok && u < sh.units; u += gridDim.x) {
-      const Unit x = unit_of(a, sh, u);
+      const Unit x = unit_of(a, sh, ends, u);
       if (t == 1 && !x.two) continue;
-      const int valid = valid_keys(a, x.b);
+      const int valid = x.valid;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < x.n; ++j, ++step) {
         uint32_t w[4];
@@ -799,6 +821,8 @@ void launch_tiles(const CrossAttnArgs& a, cudaStream_t s) {
   sh.pairs = FastDiv(pairs);
   sh.heads_kv = FastDiv(a.heads_kv);
   sh.q_tiles = FastDiv(q_tiles);
+  sh.listed = (a.kv_lens != nullptr || a.key_mask != nullptr) && a.batch <= kListed &&
+              (a.key_mask == nullptr || static_cast<int64_t>(a.batch) * a.seq_k <= kListedMask);
   const int sms = device_sm_count();
   kern<<<units < sms ? sh.units : sms, kTileThreads, Cfg::kSmemBytes, s>>>(maps, a, sh);
 }
