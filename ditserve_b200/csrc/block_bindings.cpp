@@ -239,6 +239,15 @@ PyObject* rms_norm_quant(PyObject* const* args) {
   if (scale_out.has_value() && (scale_out->sizes() != x.sizes().slice(0, x.dim() - 1) || !scale_out->is_contiguous() ||
                                 scale_out->scalar_type() != at::kFloat || scale_out->device() != dev))
     return nothing();
+  // the row's codes and scale leave while other rows are still read
+  const Rows rs{1, rx.rows, rx.rows};
+  auto clear_of = [&](const at::Tensor& t, const Rows& r) {
+    return (!out.has_value() || apart(*out, rq, t, r)) && (!scale_out.has_value() || apart(*scale_out, rs, t, r));
+  };
+  if (rx.rows > 0 && (!clear_of(x, rx) || (residual.has_value() && !clear_of(*residual, rr)) ||
+                      (residual_out.has_value() && !clear_of(*residual_out, rh)) ||
+                      (out.has_value() && scale_out.has_value() && !apart(*scale_out, rs, *out, rq))))
+    return nothing();
   if (residual.has_value()) {
     if (!residual_out.has_value()) {
       h = empty(x.sizes(), x.scalar_type(), dev);
@@ -301,6 +310,7 @@ PyObject* linear_fp8(PyObject* const* args) {
   if (out.has_value()) {
     out_type = out->scalar_type();
     if (out->sizes() != at::IntArrayRef(shape) || (N > 0 && !as_output(*out, dev, ry))) return nothing();
+    if (N > 0 && (!apart(*out, ry, x, rx) || !apart(*out, ry, w, rw))) return nothing();
   } else {
     ry.stride = N;
   }

@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             ++q_count[t];
             mbar_arrive_expect_tx(&q_full[t], Cfg::kQBytes);
             const int2 at = tile_of(a, sh, x, t);
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < Cfg::kAtoms; ++i)
               tma_load_3d(sQ + t * Cfg::kQBytes + i * (kQT * 128), &maps.q, at.x * D + i * 64, at.y,
                           sh.q_shared ? 0 : x.b, &q_full[t]);
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (!mbar_wait(&empty[st], ((count / ST) & 1) ^ 1, abort_flag, a.status, site)) return false;
           ++count;
           mbar_arrive_expect_tx(&full[st], Cfg::kKvBytes);
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < Cfg::kAtoms; ++i)
             tma_load_3d(base + st * Cfg::kKvBytes + i * (kKT * 128), map, s.x.hk * D + i * 64, s.j * kKT,
                         shared ? 0 : s.x.b, &full[st]);
@@ -601,14 +601,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tile_mask(a, s.x.b, s.j, s.x.valid, w);
           // every lane waits, so that what TMA wrote is ordered before its stores
           if (!mbar_wait_warp(&v_full[st], (vc / ST) & 1, abort_flag, a.status, 430)) break;
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (!((w[i] >> lane) & 1)) {
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < Cfg::kAtoms; ++c) {
                 // a key's 64 values are one 128-byte row of the atom, however its pieces are swizzled
                 uint4* row = reinterpret_cast<uint4*>(sV + st * Cfg::kKvBytes + c * (kKT * 128) + (i * 32 + lane) * 128);
-  #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 8; ++e) row[(e + lane) & 7] = make_uint4(0, 0, 0, 0);
               }
             }

@@ -153,8 +153,7 @@ template <typename T, int kM>
 void launch_rows(const LinearFp8Args& a, cudaStream_t s) {
   auto kern = linear_rows_kernel<T, kM>;
   constexpr int kSmem = sizeof(RowSmem<kM>);
-  static std::atomic<uint64_t> allowed{0};
-  if (kSmem > 48 * 1024) allow_smem(kern, kSmem, allowed);
+  static_assert(kSmem <= 48 * 1024, "more needs an opt-in");
   const int64_t gx = (static_cast<int64_t>(a.N) + 15) / 16, gy = (a.M + 8 * kM - 1) / (8 * kM);
   const int split = row_split(gx * gy, a.K);
   if (gx * split > 0x7fffffff) throw std::runtime_error("linear_fp8: too many channels");
@@ -175,7 +174,7 @@ void launch_rows(const LinearFp8Args& a, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------
 // Many rows: persistent, warp-specialised tcgen05 product (kind::f8f6f4).  A tile is 128 rows of x per
-// CTA and bn output channels (a multiple of 16 up to 256, a launch parameter).  Warp 0 streams 128-byte
+// CTA and bn output channels (whole 64-byte units of y up to 256, a launch parameter).  Warp 0 streams 128-byte
 // k-blocks of both operands with TMA (128-byte swizzle) through a ring of stages, warp 1 issues the
 // products into one of two TMEM accumulators, warps 2..17 scale, finish and store the other.
 // kPair: two CTAs share one 256-row tile (cta_group::2), each staging its rows of x and half of the

@@ -277,7 +277,7 @@ void launch_rows(const NormQuantArgs& a, cudaStream_t s) {
   else if (per == 1) norm_quant_kernel<T, V, 1, false><<<grid, threads, 0, s>>>(a);
   else if (per == 2) norm_quant_kernel<T, V, 2, false><<<grid, threads, 0, s>>>(a);
   else if (per == 4) norm_quant_kernel<T, V, 4, false><<<grid, threads, 0, s>>>(a);
-  else norm_quant_kernel<T, V, 8, false><<<grid, threads, 0, s>>>(a);
+  else if constexpr (V <= 2) norm_quant_kernel<T, V, 8, false><<<grid, threads, 0, s>>>(a);
 }
 
 bool aligned(const void* p, int64_t stride_bytes, int bytes) {

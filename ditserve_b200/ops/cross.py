@@ -59,14 +59,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     """softmax(scale * q k^T) v over the keys that are left of each batch entry.
 
     q [B, Sq, heads * head_dim], k and v [B, Sk, heads_kv * head_dim] in bf16 or fp16, head_dim 64 or
-    128 (2-D tensors: one batch entry); head h reads key head h // (heads / heads_kv).  kv_lens: int32
+    128 (2-D tensors: one batch entry); head h reads key head h // (heads / heads_kv); at most 65535
+    batch entries and key heads.  kv_lens: int32
     or int64 [B], the first kv_lens[b] keys are valid (held to 0 .. Sk); key_mask: bool [B, Sk], False
     keys are left out; both may be given.  What left-out slots of k and v hold does not matter, NaN and
     infinities included.  A query with no key left gets zeros and an lse of -inf.  scale > 0, 1 /
     sqrt(head_dim) by default.  Any batch and row strides of at least 16 bytes' alignment are read in
     place, others copied first; a context may be shared through a batch stride of 0 (``expand``).
     Returns out [B, Sq, heads * head_dim], with return_lse also the fp32 natural-log sums [B, heads, Sq]."""
-    heads_kv = heads_kv or heads
+    heads_kv = heads if heads_kv is None else heads_kv
     if q.is_cuda:
         got = launch("cross_attention", q, k, v, heads, heads_kv, kv_lens, key_mask, scale, out, return_lse)
         if got is not None:
@@ -84,6 +85,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         raise ValueError("q, k and v must be bf16 or fp16, all the same")
     if heads < 1 or heads_kv < 1 or heads % heads_kv:
         raise ValueError("heads must be a multiple of heads_kv")
+    if q.shape[0] > 65535 or heads_kv > 65535:
+        raise ValueError("at most 65535 batch entries and key heads")
     B, Sq, width = q.shape
     Sk, d = k.shape[1], width // heads
     if width % heads or d not in (64, 128):

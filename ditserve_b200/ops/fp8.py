@@ -86,7 +86,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
     (q, scale, h): q float8_e4m3fn [..., D] with rows on 16 bytes, scale fp32 [...] with
     y ~ q * scale[..., None], scale = max(max|y| / 448, 1e-30), and h in x's type (None without a
     residual).  The norm reads h as it is stored.  ``residual_out`` may be ``residual`` or ``x`` itself.
-    A NaN or an infinity in a row makes the row's scale and q NaN."""
+    A NaN or an infinity in a row makes the row's scale and q NaN.  Squares are summed in fp32: rows whose
+    sum(h^2) passes 3.4e38 are not represented (their q is zero)."""
     if x.is_cuda:
         got = launch("rms_norm_quant", x, weight, residual, eps, out, scale_out, residual_out)
         if got is not None:
@@ -117,6 +118,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
     x2 = x2 if x2.stride(1) == 1 or d == 1 else x2.contiguous()
     q2 = empty_fp8(x2.shape[0], d, x.device) if out is None else _rows_view(out, d, "out")
     s1 = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
+    if out is not None and any(t is not None and _partial_overlap(q2, t.reshape(-1, d)) for t in (x, residual, residual_out)):
+        raise ValueError("out overlaps the other tensors")
     if residual is not None:
         r2 = residual.reshape(-1, d)
         r2 = r2 if r2.stride(1) == 1 or d == 1 else r2.contiguous()
@@ -224,7 +227,10 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
         r2 = r2 if r2.stride(1) == 1 or N == 1 else r2.contiguous()
         if out is not None and _partial_overlap(y2, r2):
             raise ValueError("out overlaps the residual without being it")
-    got = launch("linear_fp8", _aligned_rows(xq.reshape(-1, K)), x_scale.reshape(-1).contiguous(), _aligned_rows(wq),
+    x2, w2 = _aligned_rows(xq.reshape(-1, K)), _aligned_rows(wq)
+    if out is not None and (_partial_overlap(y2, x2) or _partial_overlap(y2, w2)):
+        raise ValueError("out overlaps the operands")
+    got = launch("linear_fp8", x2, x_scale.reshape(-1).contiguous(), w2,
                  w_scale.contiguous(), b if b is None else b.contiguous(), act is not None, r2,
                  gate if gate is None or gate.stride(1) == 1 else gate.contiguous(), rows_per_batch,
                  row_batch if row_batch is None else row_batch.contiguous(), y2, out_dtype)

@@ -42,8 +42,8 @@ def rope_axes_reference(x, positions, dims, head_dim, theta, layout="interleaved
 @functools.lru_cache(maxsize=64)
 def _plan(dims: tuple, theta):
     """The frequencies of a set of axes, or None where dims or theta are wrong (the caller says how)."""
-    thetas = [float(theta)] * len(dims) if isinstance(theta, (int, float)) else [float(t) for t in theta]
-    return ext().rope_plan([int(d) for d in dims], thetas)
+    thetas = [float(theta)] * len(dims) if isinstance(theta, (int, float)) else list(theta)
+    return ext().rope_plan(list(dims), thetas)
 
 
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor | None = None, head_dim: int = 128,
@@ -58,7 +58,9 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
     elements (2i, 2i + 1), "half" pairs (i, i + sum(dims) / 2).  inverse turns the other way.  x and k
     (bf16, fp16 or fp32) may differ in heads.  out / k_out may be x / k themselves."""
     if x.is_cuda and layout in ("interleaved", "half"):
-        plan = _plan(tuple(dims), theta if isinstance(theta, (int, float)) else tuple(theta))
+        # by value: a tensor among them would be told apart by its identity
+        plan = _plan(tuple(int(d) for d in dims),
+                     theta if isinstance(theta, (int, float)) else tuple(float(t) for t in theta))
         if plan is not None:
             got = launch("rope_axes", x, k, positions, plan, head_dim, layout == "half", inverse, out, k_out)
             if got is not None:

@@ -216,3 +216,12 @@ def test_overlap_of_outputs():
     assert not over(a, a) and not over(a, b) and not over(b, a) and not over(a, torch.zeros(8, 32))
     assert over(buf[:, 16:48], a) and over(a, buf[:, 16:48]) and over(buf[1:, :32], buf[:-1, :32])
     assert over(buf[:, :32], buf[:, :32].reshape(-1)[:0].new_empty(0, 32)) is False
+
+
+@pytest.mark.parametrize("bad", [
+    lambda q, k: ops.cross_attention(q, k, k, 2, heads_kv=0),
+    lambda q, k: ops.cross_attention(q[:1].expand(65536, -1, -1), k[:1].expand(65536, -1, -1), k[:1].expand(65536, -1, -1), 2),
+])
+def test_cross_attention_refuses_counts(bad):
+    with pytest.raises(ValueError):
+        bad(torch.ones(2, 1, 128, dtype=BF), torch.ones(2, 1, 128, dtype=BF))

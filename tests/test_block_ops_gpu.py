@@ -347,3 +347,143 @@ def test_refusals_of_the_cpu_hold_on_the_device():
                 _to_dev(case)(*args[name])
                 pytest.fail(f"{name}[{i}] was not refused")
     assert ops.launch_counts() == before  # nothing ran
+
+
+# ---- more work than the device holds at once, wide strides, calls side by side ------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("B,sq,sk,heads,heads_kv,d", [
+    (8, 300, 200, 24, 24, 64), (6, 260, 333, 16, 16, 128), (5, 1024, 333, 24, 24, 64), (7, 130, 140, 30, 10, 128),
+    (4, 700, 129, 48, 16, 64)])
+def test_cross_attention_several_units_a_block(dtype, B, sq, sk, heads, heads_kv, d):
+    """Row tiles for several rounds of the device, odd counts of them, entries of every length with empty ones between."""
+    q = _randn(B, sq, heads * d, seed=1, dtype=dtype)
+    k, v = _randn(B, sk, heads_kv * d, seed=2, dtype=dtype), _randn(B, sk, heads_kv * d, seed=3, dtype=dtype)
+    lens = torch.tensor([(sk, 0, 1, sk // 2 + 1, 128, sk - 1, 0, 129)[i] for i in range(B)], device=_dev(), dtype=torch.int32)
+    mask = torch.rand(B, sk, device=_dev(), generator=torch.Generator(device=_dev()).manual_seed(4)) < 0.6
+    mask[0, sk // 3:] = False  # padding that the mask alone gives
+    valid = torch.arange(sk, device=_dev()) < lens[:, None]
+    for kw, allowed in ((dict(), valid | True), (dict(kv_lens=lens), valid), (dict(key_mask=mask), mask),
+                        (dict(kv_lens=lens, key_mask=mask), valid & mask)):
+        ki, vi = k.masked_fill(~allowed[..., None], math.nan), v.masked_fill(~allowed[..., None], math.nan)
+        o, lse = ops.cross_attention(q, ki, vi, heads, heads_kv=heads_kv, return_lse=True, **kw)
+        ops.check_status(_dev())
+        oracle.check_cross(o, lse, q, ki, vi, heads, heads_kv, allowed)
+        again = ops.cross_attention(q, ki, vi, heads, heads_kv=heads_kv, **kw)
+        assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("B,sq,sk,heads,masked", [(70, 130, 200, 1, False), (70, 130, 200, 2, True), (2, 300, 33000, 8, True)])
+def test_cross_attention_more_keys_than_a_block_lists(B, sq, sk, heads, masked):
+    q, k, v = (_randn(B, n, heads * 64, seed=s, dtype=BF) for n, s in ((sq, 1), (sk, 2), (sk, 3)))
+    lens = torch.tensor([(i * 37) % (sk + 1) for i in range(B)], device=_dev(), dtype=torch.int32)
+    lens[-1] = sk
+    allowed = torch.arange(sk, device=_dev()) < lens[:, None]
+    mask = None
+    if masked:
+        mask = torch.rand(B, sk, device=_dev(), generator=torch.Generator(device=_dev()).manual_seed(5)) < 0.5
+        mask[B // 2] = False
+        allowed = allowed & mask
+    o, lse = ops.cross_attention(q, k, v, heads, kv_lens=lens, key_mask=mask, return_lse=True)
+    ops.check_status(_dev())
+    oracle.check_cross(o, lse, q, k, v, heads, None, allowed)
+
+
+def _wide(buf, rows, cols, pitch, at, dtype, seed):
+    """[rows, cols] of ``buf`` (bytes) with rows ``pitch`` elements apart from byte ``at`` on, filled."""
+    t = buf.view(dtype).as_strided((rows, cols), (pitch, 1), at // dtype.itemsize)
+    t.copy_(_randn(rows, cols, seed=seed, dtype=FL).to(dtype))
+    return t
+
+
+def test_rows_that_lie_more_than_32_bits_apart():
+    buf = torch.empty(10 << 30, device=_dev(), dtype=torch.uint8)  # rows' last elements behind 2^32 of them
+    wide = 1 << 30
+    for rows, pitch in ((5, wide), (1200, wide >> 8)):
+        x, r, h = (_wide(buf, rows, 256, pitch, i * 1024, BF, i) for i in range(3))
+        q = _wide(buf, rows, 256, 2 * pitch, 4096, torch.float8_e4m3fn, 5)
+        want = ops.rms_norm_quant(x.contiguous(), residual=r.contiguous())
+        got = ops.rms_norm_quant(x, residual=r, residual_out=h, out=q)
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, want))
+    pos = torch.arange(5, device=_dev())
+    x, y = _wide(buf, 5, 256, wide, 0, BF, 1), _wide(buf, 5, 256, wide, 1024, BF, 2)
+    assert torch.equal(ops.rope_axes(x, pos, (64,), out=y), ops.rope_axes(x.contiguous(), pos, (64,)))
+    for m, n, cols in ((5, 5, 64), (300, 2000, 1024)):
+        pitch = wide >> (0 if m == 5 else 6)
+        x = _wide(buf, m, cols, 2 * pitch, 0, torch.float8_e4m3fn, 1)
+        w = _wide(buf, n, cols, 2 * pitch, 1024, torch.float8_e4m3fn, 2) if m == 5 else _quantised(n, 1, cols)[0]
+        sx, sw = torch.rand(m, device=_dev()), torch.rand(n, device=_dev())
+        y = _wide(buf, m, n, pitch, 4096, BF, 3)
+        want = ops.linear_fp8(x.contiguous(), sx, w.contiguous(), sw)
+        assert torch.equal(ops.linear_fp8(x, sx, w, sw, out=y), want)
+    pitch = wide >> 5
+    far = torch.empty(10 << 29, device=_dev(), dtype=BF)
+    for sq, heads in ((3, 2), (140, 20)):
+        n = heads * 128
+        k, v = (_wide(buf, 150, n, pitch, i * 8192, BF, i)[None] for i in range(2))
+        q, o = (_wide(buf, sq, n, pitch, i * 8192, BF, i)[None] for i in (2, 3))
+        want = ops.cross_attention(*(t.contiguous() for t in (q, k, v)), heads)
+        # columns of one buffer meet in their spans: the result has to lie elsewhere
+        with pytest.raises(ValueError):
+            ops.cross_attention(q, k, v, heads, out=o)
+        assert torch.equal(ops.cross_attention(q, k, v, heads, out=far.as_strided((1, sq, n), (0, pitch, 1))), want)
+    ops.check_status(_dev())
+
+
+def test_calls_side_by_side_on_two_streams():
+    """Many-tile forms on two streams at once: neither keeps anything that the other could meet."""
+    work = []
+    for seed in (0, 40):
+        q = _randn(4, 520, 12 * 64, seed=seed, dtype=BF)
+        k, v = _randn(4, 300, 12 * 64, seed=seed + 1, dtype=BF), _randn(4, 300, 12 * 64, seed=seed + 2, dtype=BF)
+        xq, xs, wq, ws = _quantised(1500, 1100, 640, seed=seed + 3)
+        a, b, c, d = _quantised(20, 256, 8192, seed=seed + 7)
+
+        def run(q=q, k=k, v=v, xq=xq, xs=xs, wq=wq, ws=ws, a=a, b=b, c=c, d=d):
+            return (ops.cross_attention(q, k, v, 12), ops.linear_fp8(xq, xs, wq, ws), ops.linear_fp8(a, b, c, d),
+                    ops.cross_attention(q[:, :2], k, v, 12), *ops.rms_norm_quant(q)[:2])
+        work.append((run, run()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[], []]
+    for _ in range(10):
+        for i, (run, _) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run())
+    torch.cuda.synchronize()
+    ops.check_status(_dev())
+    for (_, want), runs in zip(work, got):
+        for out in runs:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(out, want))
+
+
+def test_theta_is_taken_by_value():
+    x, pos = _randn(6, 128, dtype=BF), torch.arange(6, device=_dev())
+    theta = torch.tensor([100.0])
+    first = ops.rope_axes(x, pos, (64,), theta=theta)
+    assert torch.equal(first, ops.rope_axes(x, pos, (64,), theta=100.0))
+    theta.fill_(5000.0)
+    assert torch.equal(ops.rope_axes(x, pos, (64,), theta=theta), ops.rope_axes(x, pos, (64,), theta=5000.0))
+
+
+def test_outputs_on_operands_are_refused():
+    x = _randn(8, 64, dtype=BF)
+    with pytest.raises(ValueError):
+        ops.rms_norm_quant(x, out=x.view(torch.float8_e4m3fn)[:, :64])
+    h = torch.empty_like(x)
+    with pytest.raises(ValueError):
+        ops.rms_norm_quant(x, residual=x.clone(), residual_out=h, out=h.view(torch.float8_e4m3fn)[:, :64])
+    # other columns of one buffer are apart
+    buf = torch.zeros(8, 256, device=_dev(), dtype=torch.uint8)
+    xs = buf[:, :128].view(BF)
+    xs.copy_(x)
+    oracle.check_norm_quant(ops.rms_norm_quant(xs, out=buf[:, 128:192].view(torch.float8_e4m3fn)), x, None, None, 1e-6)
+    # a scale on the input is written last, through a copy
+    want = ops.rms_norm_quant(x)
+    f = x.clone()
+    q, s, _ = ops.rms_norm_quant(f, scale_out=f.view(-1)[:16].view(FL))
+    assert torch.equal(q.float(), want[0].float()) and torch.equal(s, want[1])
+    xq, sx, wq, sw = _quantised(32, 32, 64)
+    with pytest.raises(ValueError):
+        ops.linear_fp8(xq, sx, wq, sw, out=xq.view(BF))
+    with pytest.raises(ValueError):
+        ops.linear_fp8(xq, sx, wq, sw, out=wq.view(BF))
