@@ -309,7 +309,9 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 // keys take 690 us (1190 TFLOP/s), 2 x 32760 over 512 keys 205 us (1000).  Measured and not kept: P through shared memory
 // with the next scores formed during the exponentials (268 us against 240 at 4096 x 4096: operands, P and loads together
 // exceed the shared memory's rate), two threads a row (213 against 197), output warps of their own, every fourth pair of
-// exponentials as a polynomial (238 against 197), a product warp a tile (218 against 197).
+// exponentials as a polynomial (238 against 197), a product warp a tile (218 against 197), key tiles of 64 with the scores
+// formed two ahead (266 against 218; with a product warp a tile 256): a barrier's wait takes 200 cycles behind the other
+// tile's exponentials in the queue, and smaller tiles wait twice as often.
 constexpr int kQT = 128, kKT = 128, kPChunks = 2;
 constexpr int kTileThreads = 384;
 
@@ -508,15 +510,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         };
         Step cur;
         cur.u = blockIdx.x;
-        bool ok = cur.settle(a, sh, ends) && load_q(cur.x) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412);
+        // K before Q: the first tile's scores need K and that tile's Q alone
+        bool ok = cur.settle(a, sh, ends) && load_kv(cur, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412) && load_q(cur.x);
         while (ok) {
           Step next = cur;
           const bool more = next.advance(a, sh, ends);
-          // at a unit's end its last V comes before the next unit's Q, which waits for the last scores
-          const bool fresh = more && next.j == 0;
-          if (fresh && (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413) || !load_q(next.x))) break;
           if (more && !load_kv(next, &maps.k, sh.k_shared, sK, k_full, k_empty, kc, 412)) break;
-          if (!fresh && !load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
+          if (!load_kv(cur, &maps.v, sh.v_shared, sV, v_full, v_empty, vc, 413)) break;
+          // the next unit's Q, which waits for the last scores, behind all that this unit needs
+          if (more && next.j == 0 && !load_q(next.x)) break;
           cur = next;
           ok = more;
         }
