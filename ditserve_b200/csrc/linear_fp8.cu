@@ -195,6 +195,7 @@ constexpr int kSmemFixed = kEpiWarps * (kOutBytes + kColBytes) + 1024 /*align*/ 
 
 struct TileShape {
   int bn, num_m, num_n, num_k;
+  int twin;  // 1: a CTA takes two neighbouring tiles at once, one accumulator each, on the same rows of x
   int stages, stage_bytes;
   int fast;  // y and the residual have rows on 16 bytes, gate rows too: tile stores
 };
@@ -223,11 +224,11 @@ __device__ __forceinline__ float2 gelu2(float2 x) {
   return fma2(h, make_float2(tanh_approx(u.x), tanh_approx(u.y)), h);
 }
 
-// kU accumulator columns of output row m from channel n on: scale, bias, activation, gate, residual.
-// cols holds the columns' scales, then (at kCols) their biases.
+// kU accumulator columns of an output row: scale, bias, activation.  cols holds the columns' scales, then (at kCols)
+// their biases.
 template <typename T, int kU>
-__device__ __forceinline__ void finish_unit(const LinearFp8Args& a, const uint32_t (&acc)[kU], const float* cols, float sx,
-                                            int m, int n, bool row_ok, const float* gate_row, float (&v)[kU]) {
+__device__ __forceinline__ void scale_unit(const LinearFp8Args& a, const uint32_t (&acc)[kU], const float* cols, float sx,
+                                           float (&v)[kU]) {
   const float2 sx2 = make_float2(sx, sx);
 #pragma unroll
   for (int j = 0; j < kU; j += 4) {
@@ -253,6 +254,12 @@ __device__ __forceinline__ void finish_unit(const LinearFp8Args& a, const uint32
       v[j] = v[j] / (1.f + expf(-2.f * u));
     }
   }
+}
+
+// gate and residual of kU columns of output row m from channel n on; rows on 16 bytes
+template <typename T, int kU>
+__device__ __forceinline__ void add_residual(const LinearFp8Args& a, int m, int n, bool row_ok, const float* gate_row,
+                                             float (&v)[kU]) {
   if (a.residual != nullptr && row_ok) {
     constexpr int V = kVec16<T>;
     const T* r = reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n;
@@ -306,7 +313,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
   const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
-  const int tiles = sh.num_m * sh.num_n;
+  const int tiles = sh.num_m * sh.num_n, items = tiles >> sh.twin;
+  // the i-th tile of this CTA
+  auto tile_at = [&](int i) {
+    const int item = first + (i >> sh.twin) * step;
+    return item < items ? (item << sh.twin) + (i & sh.twin) : tiles;
+  };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -340,7 +352,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       uint32_t phase = 0;
       const int b_rows = sh.bn / kCtas;
       const uint32_t bytes = kCtas * sh.stage_bytes;
-      for (int tile = first; tile < tiles; tile += step) {
+      for (int item = first; item < items; item += step) {
+        const int tile = item << sh.twin;
         const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM;
         const int n0 = (tile % sh.num_n) * sh.bn + rank * b_rows;
         for (int kb = 0; kb < sh.num_k; ++kb) {
@@ -350,10 +363,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
             tma_load_2d_pair(ring + stage * sh.stage_bytes, &tmX, kb * kBK, m0, leader);
             tma_load_2d_pair(ring + stage * sh.stage_bytes + kABytes, &tmW, kb * kBK, n0, leader);
+            if (sh.twin)
+              tma_load_2d_pair(ring + stage * sh.stage_bytes + kABytes + b_rows * kBK, &tmW, kb * kBK, n0 + sh.bn, leader);
           } else {
             mbar_arrive_expect_tx(&full[stage], bytes);
             tma_load_2d(ring + stage * sh.stage_bytes, &tmX, kb * kBK, m0, &full[stage]);
             tma_load_2d(ring + stage * sh.stage_bytes + kABytes, &tmW, kb * kBK, n0, &full[stage]);
+            if (sh.twin)
+              tma_load_2d(ring + stage * sh.stage_bytes + kABytes + b_rows * kBK, &tmW, kb * kBK, n0 + sh.bn, &full[stage]);
           }
           if (++stage == ST) {
             stage = 0;
@@ -371,9 +388,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const uint32_t idesc = umma_idesc_e4m3(kCtas * kBM, sh.bn);
       int stage = 0, local = 0;
       uint32_t phase = 0;
-      for (int tile = first; tile < tiles; tile += step, ++local) {
-        const int acc = local & 1;
-        if (!mbar_wait_warp(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, a.status, 311)) goto mma_done;
+      const uint32_t twin_lo = (sh.bn / kCtas * kBK) >> 4;
+      for (int item = first; item < items; item += step, local += 1 + sh.twin) {
+        const int acc = local & 1;  // of twins the first's: 0
+        for (int g = 0; g <= sh.twin; ++g)
+          if (!mbar_wait_warp(&acc_empty[acc + g], ((local >> 1) & 1) ^ 1, abort_flag, a.status, 311)) goto mma_done;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * kMaxBn;
         for (int kb = 0; kb < sh.num_k; ++kb) {
@@ -387,6 +406,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               if constexpr (kPair) umma_f8_ss_pair(d, a_lo + 2 * k, kHi, b_lo + 2 * k, kHi, idesc, (kb | k) != 0);
               else umma_f8_ss(d, a_lo + 2 * k, kHi, b_lo + 2 * k, kHi, idesc, (kb | k) != 0);
             }
+            if (sh.twin) {
+#pragma unroll
+              for (int k = 0; k < kBK / 32; ++k) {
+                const uint32_t t_lo = b_lo + twin_lo + 2 * k;
+                if constexpr (kPair) umma_f8_ss_pair(d + kMaxBn, a_lo + 2 * k, kHi, t_lo, kHi, idesc, (kb | k) != 0);
+                else umma_f8_ss(d + kMaxBn, a_lo + 2 * k, kHi, t_lo, kHi, idesc, (kb | k) != 0);
+              }
+            }
             if constexpr (kPair) umma_commit_pair(&empty[stage]);
             else umma_commit(&empty[stage]);
           }
@@ -396,8 +423,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         if (one) {
-          if constexpr (kPair) umma_commit_pair(&acc_full[acc]);
-          else umma_commit(&acc_full[acc]);
+          for (int g = 0; g <= sh.twin; ++g) {
+            if constexpr (kPair) umma_commit_pair(&acc_full[acc + g]);
+            else umma_commit(&acc_full[acc + g]);
+          }
         }
       }
     mma_done:;
@@ -433,9 +462,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         else mbar_arrive(&acc_empty[acc]);
       }
     };
-    fetch(first);
-    int local = 0;
-    for (int tile = first; tile < tiles; tile += step, ++local) {
+    fetch(tile_at(0));
+    for (int local = 0;; ++local) {
+      const int tile = tile_at(local);
+      if (tile >= tiles) break;
       const int acc = local & 1;
       const int m0 = (tile / sh.num_n) * (kCtas * kBM) + rank * kBM + quarter * 32;
       const int m = m0 + lane;
@@ -448,7 +478,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         cols[i * 32 + lane] = p_sw[i];
         cols[kCols + i * 32 + lane] = p_b[i];
       }
-      fetch(tile + step);
+      fetch(tile_at(local + 1));
       __syncwarp();
       if (!mbar_wait_warp(&acc_full[acc], (local >> 1) & 1, abort_flag, a.status, 313)) break;
       tc_fence_after();
@@ -462,8 +492,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (c + kEpiParts * kU >= sh.bn) hand_back(acc);
         float v[kU];
         const int n = n0 + c;
-        if (sh.fast && c + kU <= sh.bn) {
-          finish_unit<T, kU>(a, r, cols + (c / kU / kEpiParts) * kU, sx, m, n, row_ok, gate_row, v);
+        scale_unit<T, kU>(a, r, cols + (c / kU / kEpiParts) * kU, sx, v);
+        if (sh.fast) {
+          add_residual<T, kU>(a, m, n, row_ok, gate_row, v);
           if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
           __syncwarp();
 #pragma unroll
@@ -476,15 +507,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (m0 < a.M && n < a.N) tma_store_2d(&tmY, n, m0, b);
             tma_store_commit();
           }
-        } else if (row_ok) {
-          // rows off 16 bytes
-          const int end = min(min(kU, sh.bn - c), a.N - n);
-          T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
+        } else {
+          // rows off 16 bytes: 16 columns at a time through the buffer, so that a warp's store is of two rows' neighbours
 #pragma unroll
-          for (int j = 0; j < kU; ++j)
-            if (j < end)
-              y[j] = from_float<T>(
-                  finish<T>(a, __uint_as_float(r[j]) * (sx * a.sw[(n + j) * a.sw_stride]), m, n + j, gate_row));
+          for (int h = 0; h < kU; h += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(b + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
+                  make_float4(v[h + 4 * q], v[h + 4 * q + 1], v[h + 4 * q + 2], v[h + 4 * q + 3]);
+            __syncwarp();
+            const int col = lane & 15, n1 = n + h + col;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 8) {  // the residuals of four stores first
+              float y[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = r0 + 2 * i + (lane >> 4);
+                const float* g = reinterpret_cast<const float*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(gate_row), k));
+                y[i] = *reinterpret_cast<const float*>(b + k * 64 + (((col >> 2) ^ ((k >> 1) & 3)) * 16) + (col & 3) * 4);
+                if (a.residual != nullptr && m0 + k < a.M && n1 < a.N)
+                  y[i] = fmaf(y[i], g != nullptr ? g[n1] : 1.f,
+                              to_float(reinterpret_cast<const T*>(a.residual)[static_cast<int64_t>(m0 + k) * a.ldr + n1]));
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = r0 + 2 * i + (lane >> 4);
+                if (m0 + k < a.M && n1 < a.N)
+                  reinterpret_cast<T*>(a.y)[static_cast<int64_t>(m0 + k) * a.ldy + n1] = from_float<T>(y[i]);
+              }
+            }
+          }
         }
       }
       if (part * kU >= sh.bn) hand_back(acc);  // a narrow tile has no unit for this warp
@@ -509,8 +563,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
+// Width of the tiles: the multiple of a unit whose rounds over the SMs cost least.  A k-block takes about 0.29 us +
+// 0.1 us * bn / 256 (8960 x 1536 channels at 32760 rows: 0.39, 0.355 and 0.325 us for 256, 192 and 128
+// channels), bound by the L2's traffic into shared memory more than by the products, so few wide rounds
+// beat many narrow ones, and a single round takes the narrowest tile that keeps it one.
+// `unit` (16 or 32) keeps whole 64-byte units of the output in a tile: the columns behind the last whole unit go out one
+// element at a time.
+// More tiles than CTAs, but fewer than twice as many: twins bring them into one round, and a k-block of x then serves
+// both (the tiles' outputs leave behind one another, which a second round would not spare either).
+struct TilePlan {
+  int bn, twin;
+  int64_t rounds;
+};
+
+TilePlan plan_tiles(int64_t num_m, int N, int slots, int unit) {
+  TilePlan best = {kMaxBn, 0, 1};
+  int64_t cost = INT64_MAX;
+  for (int twin = 0; twin < 2; ++twin) {
+    if (twin && best.rounds == 1) break;
+    for (int bn = kMaxBn; bn >= 32; bn -= unit) {
+      const int width = bn << twin;
+      const int64_t items = num_m * ((N + width - 1) / width), rounds = (items + slots - 1) / slots;
+      if (twin && rounds > 1) break;
+      const int64_t c = rounds * (width + 740);
+      if (c < cost) {
+        cost = c;
+        best = {bn, twin, rounds};
+      }
+    }
+  }
+  return best;
+}
+
 template <typename T, bool kPair>
-void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
+void launch_tiles(const LinearFp8Args& a, const TilePlan& plan, cudaStream_t s) {
+  const int bn = plan.bn;
   constexpr int kCtas = kPair ? 2 : 1;
   auto kern = linear_tile_kernel<T, kPair>;
   static std::atomic<uint64_t> allowed{0};
@@ -524,9 +611,11 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   TileShape sh;
   sh.bn = bn;
   sh.num_m = (a.M + kCtas * kBM - 1) / (kCtas * kBM);
+  sh.twin = plan.twin;
   sh.num_n = (a.N + bn - 1) / bn;
+  if (sh.twin) sh.num_n += sh.num_n & 1;  // twins are of one row of tiles
   sh.num_k = (a.K + kBK - 1) / kBK;
-  sh.stage_bytes = (kBM + bn / kCtas) * kBK;
+  sh.stage_bytes = (kBM + (bn << sh.twin) / kCtas) * kBK;
   sh.stages = std::min(kMaxStages, (kSmemBytes - kSmemFixed) / sh.stage_bytes);
   sh.fast = at(a.y, a.ldy * e, 16) && at(a.residual, a.ldr * e, 16) && at(a.gate, a.gate_stride * 4, 16);
   const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
@@ -535,7 +624,7 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   if (tiles > 0x3fffffff) throw std::runtime_error("linear_fp8: too many tiles");
   const int slots = device_sm_count() / kCtas;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCtas * static_cast<unsigned>(tiles < slots ? tiles : slots));
+  cfg.gridDim = dim3(kCtas * static_cast<unsigned>(std::min<int64_t>(tiles >> sh.twin, slots)));
   cfg.blockDim = dim3(kTileThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = s;
@@ -547,26 +636,6 @@ void launch_tiles(const LinearFp8Args& a, int bn, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, a, sh);
-}
-
-// Width of the tiles: the multiple of a unit whose rounds over the SMs cost least.  A k-block takes about 0.29 us +
-// 0.1 us * bn / 256 (8960 x 1536 channels at 32760 rows: 0.39, 0.355 and 0.325 us for 256, 192 and 128
-// channels), bound by the L2's traffic into shared memory more than by the products, so few wide rounds
-// beat many narrow ones, and a single round takes the narrowest tile that keeps it one.
-// `unit` (16 or 32) keeps whole 64-byte units of the output in a tile: the columns behind the last whole unit go out one
-// element at a time.
-int pick_bn(int64_t num_m, int N, int slots, int unit) {
-  int best = kMaxBn;
-  int64_t cost = INT64_MAX;
-  for (int bn = kMaxBn; bn >= 32; bn -= unit) {
-    const int64_t tiles = num_m * ((N + bn - 1) / bn);
-    const int64_t c = (tiles + slots - 1) / slots * (bn + 740);
-    if (c < cost) {
-      cost = c;
-      best = bn;
-    }
-  }
-  return best;
 }
 
 // Whether the few-row form takes less time, by what both were measured to take in us (in a graph, 12 to 256 rows, 64 to
@@ -581,9 +650,9 @@ bool rows_are_faster(const LinearFp8Args& a) {
   const double few = (row_split(blocks, a.K) > 1 ? 3.5 : 2.0) + static_cast<double>(blocks) * (16 + rows) * a.K / 4.8e6;
   const int m = a.M <= kBM ? kBM : 2 * kBM, slots = device_sm_count() * kBM / m;
   const int64_t num_m = (a.M + m - 1) / m;
-  const int bn = pick_bn(num_m, a.N, slots, a.out_type == kFP32 ? 16 : 32);
-  const double rounds = static_cast<double>((num_m * ((a.N + bn - 1) / bn) + slots - 1) / slots);
-  return few < 3.2 + rounds * ((a.K + kBK - 1) / kBK * (0.24 + 0.1 * bn / 256) + 0.6);
+  const TilePlan p = plan_tiles(num_m, a.N, slots, a.out_type == kFP32 ? 16 : 32);
+  const double blocks_k = static_cast<double>((a.K + kBK - 1) / kBK);
+  return few < 3.2 + static_cast<double>(p.rounds) * (blocks_k * (0.24 + 0.1 * (p.bn << p.twin) / 256) + 0.6 * (1 + p.twin));
 }
 
 template <typename T>
@@ -596,8 +665,8 @@ void launch_type(const LinearFp8Args& a, cudaStream_t s) {
   } else {
     const int sms = device_sm_count();
     constexpr int kUnit = 64 / sizeof(T);
-    if (a.M <= kBM) launch_tiles<T, false>(a, pick_bn(1, a.N, sms, kUnit), s);
-    else launch_tiles<T, true>(a, pick_bn((a.M + 2 * kBM - 1) / (2 * kBM), a.N, sms / 2, kUnit), s);
+    if (a.M <= kBM) launch_tiles<T, false>(a, plan_tiles(1, a.N, sms, kUnit), s);
+    else launch_tiles<T, true>(a, plan_tiles((a.M + 2 * kBM - 1) / (2 * kBM), a.N, sms / 2, kUnit), s);
   }
 }
 

@@ -487,3 +487,10 @@ def test_outputs_on_operands_are_refused():
         ops.linear_fp8(xq, sx, wq, sw, out=xq.view(BF))
     with pytest.raises(ValueError):
         ops.linear_fp8(xq, sx, wq, sw, out=wq.view(BF))
+
+
+@pytest.mark.parametrize("m,n,k", [(512, 10240, 4096), (513, 9001, 300), (1300, 4000, 96), (260, 19000, 130)])
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+def test_linear_fp8_twin_tiles(m, n, k, dtype):
+    """Between one and two rounds of tiles: two neighbours at once, the second behind the last channel among them."""
+    test_linear_fp8(m, n, k, dtype)
