@@ -59,8 +59,8 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
     (bf16, fp16 or fp32) may differ in heads.  out / k_out may be x / k themselves."""
     if x.is_cuda and layout in ("interleaved", "half"):
         # by value: a tensor among them would be told apart by its identity
-        plan = _plan(tuple(int(d) for d in dims),
-                     theta if isinstance(theta, (int, float)) else tuple(float(t) for t in theta))
+        plan = _plan(tuple(map(int, dims)),
+                     theta if isinstance(theta, (int, float)) else tuple(map(float, theta)))
         if plan is not None:
             got = launch("rope_axes", x, k, positions, plan, head_dim, layout == "half", inverse, out, k_out)
             if got is not None:
