@@ -12,7 +12,8 @@
 // One pass over memory: a row stays in registers between its sum of squares, its maximum and its
 // quantisation, so an element costs its own read(s), the stored h and one byte.  Bound by HBM: 32760 x 1536 in bf16
 // with a residual takes 64 us (5.5 TB/s, the rate of a copy of as many bytes); rows that start off 16 bytes go in pieces
-// of 4 bytes (1530 wide: 105 us) or single elements (1531: 148 us).
+// of 4 bytes (1530 wide: 105 us) or single elements (1531: 148 us).  Measured and not kept: cutting such rows' vectors out
+// of two aligned ones, stores put together across lanes (148 and 158 us).
 #include <cuda_fp8.h>
 
 #include "elem.cuh"
