@@ -494,3 +494,27 @@ def test_outputs_on_operands_are_refused():
 def test_linear_fp8_twin_tiles(m, n, k, dtype):
     """Between one and two rounds of tiles: two neighbours at once, the second behind the last channel among them."""
     test_linear_fp8(m, n, k, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+def test_linear_fp8_twin_tiles_of_one_block(dtype):
+    """One row of tiles for more channels than the device has blocks: twins without CTA pairs."""
+    test_linear_fp8(100, 40000, 256, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("n", [641, 1555])
+def test_linear_fp8_rows_off_16_bytes_in_place(n, dtype):
+    """Odd rows with a gated residual that is the output, inside a wider buffer."""
+    m, k = 700, 1700
+    xq, xs, wq, ws = _quantised(m, n, k)
+    buf, gate = _randn(m + 1, n + 4, seed=6, dtype=dtype), _randn(2, n, seed=7)
+    keep = buf.clone()
+    out = buf[:m, 3:n + 3]
+    rows = torch.arange(m, device=_dev()) // 400
+    want = oracle.linear(xq, xs, wq, ws, residual=out.clone(), gate_rows=gate[rows])
+    ops.linear_fp8(xq, xs, wq, ws, residual=out, gate=gate, rows_per_batch=400, out=out)
+    ops.check_status(_dev())
+    oracle.check_linear(out, *want)
+    buf[:m, 3:n + 3] = keep[:m, 3:n + 3]
+    assert torch.equal(buf, keep)
