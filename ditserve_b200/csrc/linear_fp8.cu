@@ -197,13 +197,13 @@ constexpr int kMaxBn = 256;
 constexpr int kOutBytes = 32 * 64, kCols = kMaxBn / kEpiParts, kColBytes = 2 * kCols * 4;
 constexpr int kMaxStages = 10;
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kSmemFixed = kEpiWarps * (kOutBytes + kColBytes) + 1024 /*align*/ + 256 /*barriers*/;
+constexpr int kSmemFixed = kEpiWarps * (kOutBytes + kColBytes) + 1024 /*align*/ + 512 /*barriers*/;
 
 struct TileShape {
   int bn, num_m, num_n, num_k;
   int twin;  // 1: a CTA takes two neighbouring tiles at once, one accumulator each, on the same rows of x
   int stages, stage_bytes;
-  int fast;  // y and the residual have rows on 16 bytes, gate rows too: tile stores
+  int fast;  // y and the residual have separate rows on 16 bytes, gate rows too: tile stores and loads
 };
 
 // two floats at once on the packed datapath
@@ -259,43 +259,46 @@ __device__ __forceinline__ void scale_unit(const LinearFp8Args& a, const uint32_
   }
 }
 
-// gate and residual of kU columns of output row m from channel n on; rows on 16 bytes
+// 16-byte piece q of a lane's row in a warp's staging buffer (the 64-byte swizzle's place)
+__device__ __forceinline__ uint8_t* piece(uint8_t* b, int lane, int q) {
+  return b + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16);
+}
+
+// gate and residual of kU columns from channel n on; the residual's tile lies in the staging buffer
 template <typename T, int kU>
-__device__ __forceinline__ void add_residual(const LinearFp8Args& a, int m, int n, bool row_ok, const float* gate_row,
+__device__ __forceinline__ void add_residual(const LinearFp8Args& a, uint8_t* b, int lane, int n, const float* gate_row,
                                              float (&v)[kU]) {
-  if (a.residual != nullptr && row_ok) {
-    constexpr int V = kVec16<T>;
-    const T* r = reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n;
+  constexpr int V = kVec16<T>;
+  if (gate_row != nullptr) {
 #pragma unroll
-    for (int j = 0; j < kU; j += V) {
-      if (n + j + V <= a.N) {
-        float f[V];
-        load_vec<T, V>(r + j, f);
-        if (gate_row != nullptr) {
-#pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            const float4 g = *reinterpret_cast<const float4*>(gate_row + n + j + e);
-            v[j + e] *= g.x;
-            v[j + e + 1] *= g.y;
-            v[j + e + 2] *= g.z;
-            v[j + e + 3] *= g.w;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[j + e] += f[e];
+    for (int j = 0; j < kU; j += 4) {
+      if (n + j + 4 <= a.N) {
+        const float4 g = *reinterpret_cast<const float4*>(gate_row + n + j);
+        v[j] *= g.x;
+        v[j + 1] *= g.y;
+        v[j + 2] *= g.z;
+        v[j + 3] *= g.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (n + j + e < a.N) v[j + e] = fmaf(v[j + e], gate_row != nullptr ? gate_row[n + j + e] : 1.f, to_float(r[j + e]));
+        for (int e = 0; e < 4; ++e)
+          if (n + j + e < a.N) v[j + e] *= gate_row[n + j + e];
       }
     }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float f[V];
+    load_vec<T, V>(reinterpret_cast<const T*>(piece(b, lane, q)), f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[q * V + e] += f[e];
   }
 }
 
 template <typename T, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                       const __grid_constant__ CUtensorMap tmY, LinearFp8Args a, TileShape sh) {
+                       const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR, LinearFp8Args a,
+                       TileShape sh) {
   constexpr int kCtas = kPair ? 2 : 1;
   const int ST = sh.stages;
   extern __shared__ uint8_t smem_raw[];
@@ -310,7 +313,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + 2;  // pair: the leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* res_full = acc_empty + 2;  // [epilogue warp]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + kEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -332,6 +336,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], kEpiWarps * kCtas);  // one arrival per epilogue warp
     }
+    for (int i = 0; i < kEpiWarps; ++i) mbar_init(&res_full[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -465,6 +470,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         else mbar_arrive(&acc_empty[acc]);
       }
     };
+    // the residual of the next unit comes as a tile into the staging buffer, once the last store has read it: rows read
+    // by their threads in 16-byte pieces took 64 us where this takes 46 (25528 x 768 in fp32 from 639 values)
+    const bool by_tile = sh.fast && a.residual != nullptr;
+    uint64_t* res_bar = &res_full[warp - 2];
+    uint32_t res_phase = 0;
+    auto ask = [&](int n, int m) {
+      if (lane == 0) {
+        tma_store_wait_read<0>();
+        mbar_arrive_expect_tx(res_bar, kOutBytes);
+        tma_load_2d(b, &tmR, n, m, res_bar);
+      }
+    };
     fetch(tile_at(0));
     for (int local = 0;; ++local) {
       const int tile = tile_at(local);
@@ -482,7 +499,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         cols[kCols + i * 32 + lane] = p_b[i];
       }
       fetch(tile_at(local + 1));
-      if (a.residual != nullptr && row_ok) {  // this warp's pieces of the residual are on their way into the L2 meanwhile
+      if (by_tile && part * kU < sh.bn) ask(n0 + part * kU, m0);  // on its way while the accumulator is waited for
+      if (!sh.fast && a.residual != nullptr && row_ok) {     // off 16 bytes at least on its way into the L2
         const T* res = reinterpret_cast<const T*>(a.residual) + static_cast<int64_t>(m) * a.ldr + n0;
         for (int c = part * kU; c < sh.bn && n0 + c < a.N; c += kEpiParts * kU)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(res + c));
@@ -502,12 +520,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int n = n0 + c;
         scale_unit<T, kU>(a, r, cols + (c / kU / kEpiParts) * kU, sx, v);
         if (sh.fast) {
-          add_residual<T, kU>(a, m, n, row_ok, gate_row, v);
-          if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
-          __syncwarp();
+          if (by_tile) {
+            if (!mbar_wait_warp(res_bar, res_phase, abort_flag, a.status, 314)) goto epilogue_done;
+            res_phase ^= 1;
+            add_residual<T, kU>(a, b, lane, n, gate_row, v);
+          } else {
+            if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
+            __syncwarp();
+          }
 #pragma unroll
-          for (int q = 0; q < 4; ++q)  // 16-byte pieces in the 64-byte swizzle's places
-            store_vec<T, kVec16<T>>(reinterpret_cast<T*>(b + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)),
+          for (int q = 0; q < 4; ++q)
+            store_vec<T, kVec16<T>>(reinterpret_cast<T*>(piece(b, lane, q)),
                                     *reinterpret_cast<const float(*)[kVec16<T>]>(&v[q * kVec16<T>]));
           fence_proxy_async_smem();
           __syncwarp();
@@ -515,6 +538,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (m0 < a.M && n < a.N) tma_store_2d(&tmY, n, m0, b);
             tma_store_commit();
           }
+          if (by_tile && c + kEpiParts * kU < sh.bn) ask(n + kEpiParts * kU, m0);
         } else {
           // rows off 16 bytes: 16 columns at a time through the buffer, so that a warp's store is of two rows' neighbours
 #pragma unroll
@@ -551,6 +575,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (part * kU >= sh.bn) hand_back(acc);  // a narrow tile has no unit for this warp
     }
+  epilogue_done:
     if (lane == 0) tma_store_wait_all();
   }
 
@@ -627,9 +652,14 @@ void launch_tiles(const LinearFp8Args& a, const TilePlan& plan, cudaStream_t s) 
   sh.num_k = (a.K + kBK - 1) / kBK;
   sh.stage_bytes = (kBM + (bn << sh.twin) / kCtas) * kBK;
   sh.stages = std::min(kMaxStages, (kSmemBytes - kSmemFixed) / sh.stage_bytes);
-  sh.fast = at(a.y, a.ldy * e, 16) && at(a.residual, a.ldr * e, 16) && at(a.gate, a.gate_stride * 4, 16);
+  sh.fast = at(a.y, a.ldy * e, 16) && at(a.residual, a.ldr * e, 16) && at(a.gate, a.gate_stride * 4, 16) &&
+            (a.residual == nullptr || a.ldr >= a.N);
   const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
   const CUtensorMap tmY = sh.fast ? make_tmap_out_2d(a.y, type, sizeof(T), a.M, a.N, a.ldy, 32) : tmX;
+  const CUtensorMap tmR =
+      sh.fast && a.residual != nullptr
+          ? make_tmap_out_2d(const_cast<void*>(a.residual), type, sizeof(T), a.M, a.N, a.ldr, 32)
+          : tmX;
   const int64_t tiles = static_cast<int64_t>(sh.num_m) * sh.num_n;
   if (tiles > 0x3fffffff) throw std::runtime_error("linear_fp8: too many tiles");
   const int slots = device_sm_count() / kCtas;
@@ -645,7 +675,7 @@ void launch_tiles(const LinearFp8Args& a, const TilePlan& plan, cudaStream_t s) 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, a, sh);
+  cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, tmR, a, sh);
 }
 
 // Whether the few-row form takes less time, by what both were measured to take in us (in a graph, 12 to 256 rows, 64 to

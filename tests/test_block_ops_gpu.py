@@ -518,3 +518,15 @@ def test_linear_fp8_rows_off_16_bytes_in_place(n, dtype):
     oracle.check_linear(out, *want)
     buf[:m, 3:n + 3] = keep[:m, 3:n + 3]
     assert torch.equal(buf, keep)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL])
+def test_linear_fp8_broadcast_residual(dtype):
+    """One row of residual for all rows (a stride of 0), and rows of it that overlap."""
+    m, n, k = 400, 1024, 1500
+    xq, xs, wq, ws = _quantised(m, n, k)
+    flat = _randn(n + 8 * m, seed=6, dtype=dtype)
+    for r in (flat[:n].expand(m, n), flat.as_strided((m, n), (8, 1))):
+        y = ops.linear_fp8(xq, xs, wq, ws, residual=r, out_dtype=dtype)
+        ops.check_status(_dev())
+        oracle.check_linear(y, *oracle.linear(xq, xs, wq, ws, residual=r))
