@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 from ._ext import launch, status_word, use_kernels
+from ._memory import shares_memory
 from .gemm import _row_gate, gelu_tanh_ref
 
 E4M3 = torch.float8_e4m3fn
@@ -85,7 +86,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
     x: [..., D] in bf16, fp16 or fp32, any row stride; weight [D] in the same type.  Returns
     (q, scale, h): q float8_e4m3fn [..., D] with rows on 16 bytes, scale fp32 [...] with
     y ~ q * scale[..., None], scale = max(max|y| / 448, 1e-30), and h in x's type (None without a
-    residual).  The norm reads h as it is stored.  ``residual_out`` may be ``residual`` or ``x`` itself.
+    residual).  The norm reads h as it is stored.  ``residual_out`` may be ``residual`` or ``x`` itself; the
+    outputs share no memory with each other (columns of one buffer are apart).
     A NaN or an infinity in a row makes the row's scale and q NaN.  Squares are summed in fp32: rows whose
     sum(h^2) passes 3.4e38 are not represented (their q is zero)."""
     if x.is_cuda:
@@ -107,6 +109,9 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
         raise ValueError("out must be float8_e4m3fn of x's shape")
     if scale_out is not None and (scale_out.shape != shape[:-1] or scale_out.dtype != torch.float32):
         raise ValueError("scale_out must be fp32 of x's shape without its last axis")
+    outs = [t for t in (out, scale_out, residual_out) if t is not None]
+    if any(shares_memory(a, b) for i, a in enumerate(outs) for b in outs[i + 1:]):
+        raise ValueError("out, scale_out and residual_out must not share memory")
     if not use_kernels(x, weight, residual, out, scale_out, residual_out):
         q, s, h = rms_norm_quant_reference(x, weight, residual, eps)
         q = q if out is None else out.copy_(q)
