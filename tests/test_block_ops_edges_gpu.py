@@ -32,3 +32,35 @@ def test_rms_norm_quant_outputs_share_no_memory(case):
 def test_rms_norm_quant_scale_beside_the_codes():
     x = _randn(8, 64, dtype=BF)
     oracle.check_norm_quant(cpu.scale_on_other_outputs(_dev())[1](x), x, None, None, 1e-6)
+
+
+# ---- linear_fp8 -------------------------------------------------------------------------------
+def gelu_cases(m, dtype):
+    """Every row and column of the product is one pre-activation, exactly: 1 * 1 * its channel's scale."""
+    t = torch.cat([torch.linspace(-12, 12, 8193), torch.linspace(-40, 40, 801),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e4, -1e4, 6e4, -6e4])]).to(_dev())
+    one = torch.zeros(m, 64, device=_dev())
+    one[:, 0] = 1
+    each = torch.zeros(t.numel(), 64, device=_dev())
+    each[:, 0] = 1
+    return t, ops.linear_fp8(one.to(E4M3), torch.ones(m, device=_dev()), each.to(E4M3), t, act="gelu", out_dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+@pytest.mark.parametrize("m", [1, 12, 100, 300])
+def test_linear_fp8_gelu_keeps_its_tail(m, dtype):
+    """x / (1 + exp(-a)), a = 2 sqrt(2/pi) (x + 0.044715 x^3), in the few-row form and in single and paired tiles.
+
+    With w = 2^-24 an fp32 rounding: the exponent takes 7 roundings, which the power turns into 7 |a| w of itself; the
+    power and the quotient err by 2^-22 each, the sum by w: (7 |a| + 9) w of the value.
+    Then the output's rounding, half a step of the smallest number in fp16, and what a power below 2^-126 leaves."""
+    t, y = gelu_cases(m, dtype)
+    ops.check_status(_dev())
+    x, w = t.double(), 2.0 ** -24
+    a = 2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+    want = x / (1 + torch.exp(-a))
+    bound = want.abs() * ((7 * a.abs() + 9) * w + oracle.u(dtype) * 1.001) + (1 + x.abs()) * 2.0 ** -126
+    if dtype == HF:
+        bound = bound + 2.0 ** -25
+    d = (y.double() - want).abs()
+    assert (d <= bound).all(), (d / bound).max()
