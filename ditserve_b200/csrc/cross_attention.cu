@@ -736,7 +736,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int2 at = tile_of(a, sh, x, t);
       const int i_q = at.y + row;
       const bool row_ok = i_q < a.seq_q;
-      const float inv = m_run == -INFINITY ? 0.f : 1.f / l_run;  // no key: zeros
+      // no key left: zeros and -inf.  A row of NaN scores has no maximum either, but a sum of NaN, which is its result
+      const bool none = m_run == -INFINITY && l_run == 0.f;
+      const float inv = none ? 0.f : 1.f / l_run;
       if (x.n > 0) {
         if (!mbar_wait_warp(&pv_done[t], (step - 1) & 1, abort_flag, a.status, 444 + t)) break;
         tc_fence_after();
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (row_ok && a.lse != nullptr)
         a.lse[(static_cast<int64_t>(x.b) * a.heads + at.x) * a.seq_q + i_q] =
-            m_run == -INFINITY ? -INFINITY : m_run * a.scale + logf(l_run);
+            none ? -INFINITY : m_run * a.scale + logf(l_run);
     }
     if (lane == 0) tma_store_wait_all();
   }

@@ -63,3 +63,34 @@ def test_rms_norm_quant_outputs_share_no_memory(case):
 def test_rms_norm_quant_scale_beside_the_codes():
     x = torch.randn(8, 64).to(BF)
     oracle.check_norm_quant(scale_on_other_outputs("cpu")[1](x), x, None, None, 1e-6)
+
+
+def nan_inputs(dev, sq, d, dtype):
+    """q, k, v of two entries with 24 heads, 300 keys, lengths and a mask; a NaN query in entry 0, a NaN key that is
+    left out in entry 0 and one that is not in head 5 of entry 1."""
+    g = torch.Generator().manual_seed(sq)
+    q, k, v = (torch.randn(2, n, 24 * d, generator=g).to(dtype) for n in (sq, 300, 300))
+    q[0, sq // 2, 3 * d + 1] = math.nan
+    k[0, 280] = math.nan
+    k[1, 130, 5 * d:6 * d] = math.nan
+    mask = torch.ones(2, 300, dtype=torch.bool)
+    mask[:, 5:9] = False
+    return (*(t.to(dev) for t in (q, k, v)), torch.tensor([270, 200], device=dev, dtype=torch.int32), mask.to(dev))
+
+
+def check_nan(o, lse, o_want, lse_want, sq, d):
+    """NaN exactly where a query, or a key that it may attend to, is NaN: outputs and log sums, in that head alone."""
+    nan = torch.zeros(2, 24, sq, dtype=torch.bool)
+    nan[0, 3, sq // 2] = True
+    nan[1, 5] = True
+    assert torch.equal(lse_want.isnan().cpu(), nan) and torch.equal(lse.isnan().cpu(), nan)
+    rows = nan.transpose(1, 2)[..., None].expand(2, sq, 24, d).reshape(2, sq, 24 * d)
+    assert torch.equal(o_want.isnan().cpu(), rows) and torch.equal(o.isnan().cpu(), rows)
+    assert not lse.isinf().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_cross_attention_nan_rows(dtype):
+    q, k, v, lens, mask = nan_inputs("cpu", 3, 64, dtype)
+    got = ops.cross_attention(q, k, v, 24, kv_lens=lens, key_mask=mask, return_lse=True)
+    check_nan(*got, *got, 3, 64)

@@ -64,3 +64,15 @@ def test_linear_fp8_gelu_keeps_its_tail(m, dtype):
         bound = bound + 2.0 ** -25
     d = (y.double() - want).abs()
     assert (d <= bound).all(), (d / bound).max()
+
+
+# ---- cross_attention --------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq", [3, 520])  # few-row form, tiles
+def test_cross_attention_nan_rows(sq, d, dtype):
+    q, k, v, lens, mask = cpu.nan_inputs(_dev(), sq, d, dtype)
+    want = ops.cross_attention_reference(q, k, v, 24, kv_lens=lens, key_mask=mask, return_lse=True)
+    got = ops.cross_attention(q, k, v, 24, kv_lens=lens, key_mask=mask, return_lse=True)
+    ops.check_status(_dev())
+    cpu.check_nan(*got, *want, sq, d)
