@@ -15,6 +15,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 
@@ -511,7 +512,8 @@ PyObject* cross_attention(PyObject* const* args) {
     a.mask_col = m.stride(1);
   }
   const double s = args[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : float_arg(args[7]);
-  if (!(s > 0.0) || !std::isfinite(s)) return nothing();
+  // the kernels multiply scores, -inf among them, by scale * log2(e) in fp32: neither zero nor infinite there
+  if (!(s >= FLT_TRUE_MIN) || !(s * M_LOG2E <= FLT_MAX)) return nothing();
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor o = out.has_value() ? *out : empty(q.sizes(), q.scalar_type(), dev), lse;
   if (return_lse) {

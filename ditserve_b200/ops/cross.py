@@ -13,6 +13,9 @@ import torch
 
 from ._ext import launch, status_word, use_kernels
 
+# fp32's smallest number; its largest over log2(e), which the exponentials' base takes in
+SCALE_MIN, SCALE_MAX = 2.0 ** -149, torch.finfo(torch.float32).max / math.log2(math.e)
+
 
 def cross_attention_reference(q, k, v, heads, heads_kv=None, kv_lens=None, key_mask=None, scale=None, return_lse=False):
     """fp32 PyTorch statement of the op for [B, S, heads * head_dim] tensors (CPU path and test oracle)."""
@@ -63,8 +66,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     batch entries and key heads.  kv_lens: int32
     or int64 [B], the first kv_lens[b] keys are valid (held to 0 .. Sk); key_mask: bool [B, Sk], False
     keys are left out; both may be given.  What left-out slots of k and v hold does not matter, NaN and
-    infinities included.  A query with no key left gets zeros and an lse of -inf.  scale > 0, 1 /
-    sqrt(head_dim) by default.  Any batch and row strides of at least 16 bytes' alignment are read in
+    infinities included.  A query with no key left gets zeros and an lse of -inf.  scale is positive, 2^-149 to
+    2.3e38, 1 / sqrt(head_dim) by default.  Any batch and row strides of at least 16 bytes' alignment are read in
     place, others copied first; a context may be shared through a batch stride of 0 (``expand``).
     Returns out [B, Sq, heads * head_dim], with return_lse also the fp32 natural-log sums [B, heads, Sq]."""
     heads_kv = heads if heads_kv is None else heads_kv
@@ -98,8 +101,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     if key_mask is not None and (key_mask.shape != (B, Sk) or key_mask.dtype != torch.bool):
         raise ValueError(f"key_mask must be bool [{B}, {Sk}]")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError("scale must be positive and finite")
+    if not SCALE_MIN <= scale <= SCALE_MAX:
+        raise ValueError("scale must be positive and finite in fp32, and so must scale * log2(e)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise ValueError("out must have q's shape and type")
     if out is not None and any(_shares_memory(out, t) for t in (q, k, v)):

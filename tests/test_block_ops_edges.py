@@ -94,3 +94,20 @@ def test_cross_attention_nan_rows(dtype):
     q, k, v, lens, mask = nan_inputs("cpu", 3, 64, dtype)
     got = ops.cross_attention(q, k, v, 24, kv_lens=lens, key_mask=mask, return_lse=True)
     check_nan(*got, *got, 3, 64)
+
+
+BAD_SCALES = [0.0, -0.5, 1e-50, 1e-45, 3e38, 1e39, math.inf, math.nan]
+
+
+@pytest.mark.parametrize("scale", BAD_SCALES)
+def test_cross_attention_scales_out_of_range(scale):
+    q = torch.ones(1, 2, 64, dtype=BF)
+    with pytest.raises(ValueError):
+        ops.cross_attention(q, q, q, 1, scale=scale)
+
+
+def test_cross_attention_smallest_scale():
+    q, k, v = (torch.randn(2, n, 128).to(BF) for n in (3, 20, 20))
+    lens = torch.tensor([20, 7], dtype=torch.int32)
+    o, lse = ops.cross_attention(q, k, v, 2, kv_lens=lens, scale=2e-45, return_lse=True)
+    oracle.check_cross(o, lse, q, k, v, 2, allowed=torch.arange(20) < lens[:, None], scale=2e-45)

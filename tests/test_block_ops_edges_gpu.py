@@ -76,3 +76,29 @@ def test_cross_attention_nan_rows(sq, d, dtype):
     got = ops.cross_attention(q, k, v, 24, kv_lens=lens, key_mask=mask, return_lse=True)
     ops.check_status(_dev())
     cpu.check_nan(*got, *want, sq, d)
+
+
+@pytest.mark.parametrize("sq", [3, 520])
+def test_cross_attention_scales_out_of_range(sq):
+    """Refused, in both forms; the smallest scale is a plain mean over the keys that are left."""
+    q, k, v = (_randn(2, n, 24 * 64, seed=s, dtype=BF) for n, s in ((sq, 1), (300, 2), (300, 3)))
+    lens = torch.tensor([270, 131], device=_dev(), dtype=torch.int32)
+    before = ops.launch_counts()
+    for scale in cpu.BAD_SCALES:
+        with pytest.raises(ValueError):
+            ops.cross_attention(q, k, v, 24, kv_lens=lens, scale=scale)
+            pytest.fail(f"{scale} was not refused")
+    assert ops.launch_counts() == before
+    o, lse = ops.cross_attention(q, k, v, 24, kv_lens=lens, scale=2e-45, return_lse=True)
+    ops.check_status(_dev())
+    oracle.check_cross(o, lse, q, k, v, 24, allowed=torch.arange(300, device=_dev()) < lens[:, None], scale=2e-45)
+
+
+@pytest.mark.parametrize("sq", [3, 520])
+def test_cross_attention_rows_that_overlap(sq):
+    """Sliding windows over one buffer: rows 8 elements apart, read in place by loads and by tiles."""
+    flat = _randn(24 * 64 + 8 * 600, seed=5, dtype=BF)
+    q, k, v = (flat[o:].as_strided((2, n, 24 * 64), (16, 8, 1)) for o, n in ((0, sq), (8, 300), (32, 300)))
+    want = ops.cross_attention(q.contiguous(), k.contiguous(), v.contiguous(), 24)
+    assert torch.equal(ops.cross_attention(q, k, v, 24), want)
+    ops.check_status(_dev())
