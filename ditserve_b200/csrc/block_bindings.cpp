@@ -114,6 +114,25 @@ void bind_status(const at::Tensor& word) {
   status_words[i] = word;
 }
 
+// A device's status word, cleared.  It lives as long as the process, so it comes from neither the stream that asks
+// for it nor the allocator: made while that stream is captured, a tensor would be part of the graph, whose every
+// replay would clear it again and with it what other launches reported.
+at::Tensor new_status(int64_t index) {
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  void* word = nullptr;
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaMalloc(&word, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, 2 * sizeof(int), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (s != nullptr) cudaStreamDestroy(s);
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  C10_CUDA_CHECK(e);
+  return at::from_blob(word, {2}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, static_cast<c10::DeviceIndex>(index)));
+}
+
 int* status_of(const at::Device& dev) {
   std::lock_guard<std::mutex> lock(status_mu);
   const size_t i = static_cast<size_t>(dev.index());
@@ -551,6 +570,7 @@ void add_entry(pybind11::module_& m, const char* name, const char* doc) {
 }  // namespace
 
 void bind_block_ops(pybind11::module_& m) {
+  m.def("new_status", &new_status, "a cleared status word of a device, outside of streams and graphs");
   m.def("bind_status", &bind_status, "names a device's status word to the block operators");
   py::class_<RopePlan>(m, "RopePlan");
   m.def("rope_plan", &rope_plan, "the frequencies of a set of axes, or None");

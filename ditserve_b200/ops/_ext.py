@@ -127,9 +127,11 @@ def status_word(device: torch.device) -> torch.Tensor:
         with _lock:
             buf = _status.get(idx)
             if buf is None:
-                buf = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
                 if module is not None:
+                    buf = module.new_status(idx)  # also while a stream is captured
                     module.bind_status(buf)
+                else:
+                    buf = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
                 _status[idx] = buf
     return buf
 

@@ -1,5 +1,8 @@
 """Calls of the block operators at the edge of what they take, on the GPU."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -102,3 +105,37 @@ def test_cross_attention_rows_that_overlap(sq):
     want = ops.cross_attention(q.contiguous(), k.contiguous(), v.contiguous(), 24)
     assert torch.equal(ops.cross_attention(q, k, v, 24), want)
     ops.check_status(_dev())
+
+
+# ---- graphs -----------------------------------------------------------------------------------
+_FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from ditserve_b200 import ops
+dev = torch.device("cuda", 0)
+q, k = torch.randn(1, 300, 1536, device=dev).bfloat16(), torch.randn(1, 200, 1536, device=dev).bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.cross_attention(q, k, k, 24)
+ops.check_status(dev)                  # clear before any replay
+graph.replay()
+assert torch.equal(out, ops.cross_attention(q, k, k, 24))
+word = ops.status_word(dev)
+word.fill_(1)                          # as a launch that gave up leaves it
+graph.replay()
+try:
+    ops.check_status(dev)
+except ops.KernelTimeout:
+    print("kept")
+ops.check_status(dev)                  # the report was taken
+del graph, out
+torch.cuda.empty_cache()
+ops.check_status(dev)
+"""
+
+
+def test_status_word_made_in_a_capture_outlives_replays():
+    """The first call of a process inside a capture: no replay clears what another launch reported."""
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL_IN_A_CAPTURE], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout.strip() == "kept", r.stdout + r.stderr
