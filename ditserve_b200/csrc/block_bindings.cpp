@@ -181,10 +181,10 @@ bool is_vector(const at::Tensor& t, const at::Device& dev, int64_t n, at::Scalar
   return t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.device() == dev && (n <= 1 || t.stride(0) == 1);
 }
 
-// whether `out` (rows o) shares no byte with `in` (rows i): other storages, spans that do not meet, or other
-// columns of one buffer
+// whether `out` (rows o) shares no byte with `in` (rows i): spans that do not meet, or other columns of one buffer.
+// By addresses, since a storage may be another's memory (DLPack).
 bool apart(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Rows& i) {
-  if (!out.is_alias_of(in) || o.rows == 0 || i.rows == 0) return true;
+  if (o.rows == 0 || i.rows == 0) return true;
   const int64_t eo = out.element_size(), ei = in.element_size();
   const int64_t lo = reinterpret_cast<int64_t>(out.data_ptr()), at = reinterpret_cast<int64_t>(in.data_ptr());
   const int64_t hi = lo + ((o.rows - 1) * o.stride + o.cols) * eo, end = at + ((i.rows - 1) * i.stride + i.cols) * ei;

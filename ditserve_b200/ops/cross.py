@@ -40,8 +40,8 @@ def cross_attention_reference(q, k, v, heads, heads_kv=None, kv_lens=None, key_m
 
 
 def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the spans of two tensors in one storage meet (columns of one buffer count as meeting)."""
-    if not a.numel() or not b.numel() or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+    """Whether the spans of two tensors meet (columns of one buffer count as meeting)."""
+    if not a.numel() or not b.numel() or a.device != b.device:
         return False
 
     def span(t):

@@ -61,21 +61,9 @@ def _rows_view(t: torch.Tensor, width: int, name: str) -> torch.Tensor:
 
 def _partial_overlap(out: torch.Tensor, src: torch.Tensor) -> bool:
     """Whether ``out`` shares memory with ``src`` other than element by element (both 2-D rows)."""
-    if out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr() or not out.numel() or not src.numel():
-        return False
-    e = src.element_size()
-    if out.data_ptr() == src.data_ptr() and out.element_size() == e and (out.shape[0] <= 1 or out.stride(0) == src.stride(0)):
-        return False
-    lo, hi = out.data_ptr(), out.data_ptr() + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
-    a, b = src.data_ptr(), src.data_ptr() + ((src.shape[0] - 1) * src.stride(0) + src.shape[1]) * e
-    if hi <= a or b <= lo:
-        return False
-    pitch = src.stride(0) * e
-    if pitch and out.stride(0) * out.element_size() == pitch:
-        # columns of one buffer: apart if neither range of columns wraps into the other
-        d = (lo - a) % pitch
-        return d < src.shape[1] * e or d + out.shape[1] * out.element_size() > pitch
-    return True
+    same = out.data_ptr() == src.data_ptr() and out.element_size() == src.element_size() and out.shape == src.shape and \
+        (out.shape[0] <= 1 or out.stride(0) == src.stride(0))
+    return not same and shares_memory(out, src)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,

@@ -111,3 +111,38 @@ def test_cross_attention_smallest_scale():
     lens = torch.tensor([20, 7], dtype=torch.int32)
     o, lse = ops.cross_attention(q, k, v, 2, kv_lens=lens, scale=2e-45, return_lse=True)
     oracle.check_cross(o, lse, q, k, v, 2, allowed=torch.arange(20) < lens[:, None], scale=2e-45)
+
+
+def other_storage(t):
+    """The same memory as a storage of its own."""
+    got = torch.from_dlpack(t)
+    assert got.data_ptr() == t.data_ptr() and not torch._C._is_alias_of(got, t)
+    return got
+
+
+def outputs_through_another_storage(dev):
+    """Calls whose output lies on an operand's rows, but for one: known by address alone."""
+    x, wide = torch.ones(4, 64, dtype=BF, device=dev), torch.ones(6, 64, dtype=BF, device=dev)
+    pos = torch.arange(4, device=dev)
+    xq, xs = ops.quantize_rows_fp8(torch.ones(4, 64, device=dev))
+    wq, ws = ops.quantize_rows_fp8(torch.ones(32, 64, device=dev))
+    r = torch.ones(6, 32, dtype=BF, device=dev)
+    q = torch.ones(1, 6, 64, dtype=BF, device=dev)
+    return [lambda: ops.rms_norm_quant(x, residual=wide[:4], residual_out=other_storage(wide[1:])[:4]),
+            lambda: ops.linear_fp8(xq, xs, wq, ws, residual=r[:4], out=other_storage(r[1:])[:4]),
+            lambda: ops.rope_axes(wide[:4], pos, (64,), head_dim=64, out=other_storage(wide[1:])[:4]),
+            lambda: ops.cross_attention(q[:, :4], x[None], x[None], 1, out=other_storage(q[:, 1:])[:, :4])]
+
+
+def test_overlap_is_told_by_addresses():
+    from ditserve_b200.ops.cross import _shares_memory
+    from ditserve_b200.ops.fp8 import _partial_overlap
+    buf = torch.zeros(8, 96)
+    for view in (buf[1:], buf[:, 16:48], buf.view(-1)[8:200]):
+        far = other_storage(view)
+        assert shares_memory(far, buf[:, :32]) and _shares_memory(far, buf[:, :32])
+        assert not _partial_overlap(far, view) and not _partial_overlap(view, far)
+    assert _partial_overlap(other_storage(buf[1:])[:, :32], buf[:-1, :32])
+    assert not _partial_overlap(other_storage(buf)[:, :32], buf[:, 32:])
+    with pytest.raises(ValueError):
+        outputs_through_another_storage("cpu")[3]()

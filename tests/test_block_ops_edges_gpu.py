@@ -139,3 +139,17 @@ def test_status_word_made_in_a_capture_outlives_replays():
     r = subprocess.run([sys.executable, "-c", _FIRST_CALL_IN_A_CAPTURE], capture_output=True, text=True, timeout=300,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0 and r.stdout.strip() == "kept", r.stdout + r.stderr
+
+
+# ---- outputs on other tensors -----------------------------------------------------------------
+@pytest.mark.parametrize("case", range(4))
+def test_overlap_is_told_by_addresses(case):
+    with pytest.raises(ValueError):
+        cpu.outputs_through_another_storage(_dev())[case]()
+
+
+def test_in_place_through_another_storage():
+    x, r = _randn(8, 64, dtype=BF), _randn(8, 64, seed=1, dtype=BF)
+    want = r.clone()
+    got = ops.rms_norm_quant(x, residual=r, residual_out=cpu.other_storage(r))
+    oracle.check_norm_quant((got[0], got[1], r), x, None, want, 1e-6)
