@@ -189,10 +189,16 @@ bool apart(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Row
   const int64_t lo = reinterpret_cast<int64_t>(out.data_ptr()), at = reinterpret_cast<int64_t>(in.data_ptr());
   const int64_t hi = lo + ((o.rows - 1) * o.stride + o.cols) * eo, end = at + ((i.rows - 1) * i.stride + i.cols) * ei;
   if (hi <= at || end <= lo) return true;
-  const int64_t pitch = i.stride * ei;
-  if (pitch <= 0 || o.stride * eo != pitch) return false;
+  // a single row counts as one of the other's
+  const int64_t pitch = o.rows > 1 ? o.stride * eo : i.stride * ei;
+  if (pitch <= 0 || (o.rows > 1 && i.rows > 1 && i.stride * ei != pitch) || (o.rows == 1 && i.rows == 1)) return false;
   const int64_t d = ((lo - at) % pitch + pitch) % pitch;
   return d >= i.cols * ei && d + o.cols * eo <= pitch;
+}
+
+// ... the same for a vector of `n` elements that lie together
+bool apart_from_vector(const at::Tensor& out, const Rows& o, const at::Tensor& in, int64_t n) {
+  return n == 0 || apart(out, o, in, Rows{1, n, n});
 }
 
 // ... or is `in` itself, element by element
@@ -365,6 +371,15 @@ PyObject* linear_fp8(PyObject* const* args) {
     } else if ((M + per - 1) / per > batches) {
       return nothing();
     }
+  }
+  // blocks read these while others store
+  if (out.has_value() && N > 0) {
+    if (!apart_from_vector(*out, ry, sx, M) || !apart_from_vector(*out, ry, sw, N) ||
+        (bias.has_value() && !apart_from_vector(*out, ry, *bias, N)))
+      return nothing();
+    if (gate.has_value() && (!apart(*out, ry, *gate, Rows{a.gate_stride == 0 ? 1 : a.batches, N, a.gate_stride}) ||
+                             (row_batch.has_value() && !apart_from_vector(*out, ry, *row_batch, M))))
+      return nothing();
   }
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor y = out.has_value() ? *out : empty(shape, out_type, dev);

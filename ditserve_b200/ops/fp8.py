@@ -162,7 +162,8 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     xq: float8_e4m3fn [..., K] with fp32 x_scale [...]; wq float8_e4m3fn [N, K] with fp32 w_scale [N]
     (``quantize_rows_fp8``).  Any M, N and K; rows that do not start on 16 bytes (K not a multiple
     of 16 in a packed matrix) are copied first on every call, which ``empty_fp8`` avoids.  The result, b and residual share
-    ``out_dtype`` (bf16, fp16 or fp32; ``out`` decides if given).  ``out`` may be ``residual`` itself.
+    ``out_dtype`` (bf16, fp16 or fp32; ``out`` decides if given).  ``out`` may be ``residual`` itself, but shares no memory
+    with what else is read (columns of one buffer are apart).
     gate is fp32 [N] or [B, N] and needs a residual; row m takes gate row m // rows_per_batch, or
     row_batch[m] (entries outside [0, B) take the nearest row)."""
     if xq.is_cuda and act in (None, "gelu"):
@@ -206,6 +207,9 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
                 raise ValueError(f"row_batch must be int32 [{M}]")
         elif rows_per_batch is not None and (rows_per_batch < 1 or -(-M // rows_per_batch) > gate.shape[0]):
             raise ValueError("rows_per_batch must be positive and gate have a row for every batch")
+    if out is not None and any(t is not None and shares_memory(out, t) for t in (
+            x_scale, w_scale, b, gate, row_batch if gate is not None else None)):
+        raise ValueError("out must not share memory with scales, b, gate or row_batch")
     if not use_kernels(xq, wq, x_scale, w_scale, b, residual, gate, out):
         if row_batch is not None and gate is not None:
             row_batch = row_batch.clamp(0, gate.shape[0] - 1)

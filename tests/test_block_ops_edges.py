@@ -146,3 +146,42 @@ def test_overlap_is_told_by_addresses():
     assert not _partial_overlap(other_storage(buf)[:, :32], buf[:, 32:])
     with pytest.raises(ValueError):
         outputs_through_another_storage("cpu")[3]()
+
+
+def linear_outputs_on_parameters(dev):
+    """(calls whose out lies on a scale, the bias, the gate or row_batch; one whose parameters lie beside out's rows)"""
+    xq, xs = ops.quantize_rows_fp8(torch.randn(32, 64).to(dev))
+    wq, ws = ops.quantize_rows_fp8(torch.randn(32, 64).to(dev))
+    o, r = torch.zeros(40, 32, device=dev), torch.zeros(32, 32, device=dev)
+    one = torch.ones(2, 32, device=dev)
+    refused = [lambda: ops.linear_fp8(xq, o.view(-1)[:32], wq, ws, out=o[:32]),
+               lambda: ops.linear_fp8(xq, o[:32, 5], wq, ws, out=o[:32]),
+               lambda: ops.linear_fp8(xq, xs, wq, o[31], out=o[:32]),
+               lambda: ops.linear_fp8(xq, xs, wq, ws, o[7], out=o[:32]),
+               lambda: ops.linear_fp8(xq, xs, wq, ws, residual=r, gate=o[31:33], rows_per_batch=16, out=o[:32]),
+               lambda: ops.linear_fp8(xq, xs, wq, ws, residual=r, gate=o[31], out=o[:32]),
+               lambda: ops.linear_fp8(xq, xs, wq, ws, residual=r, gate=one, row_batch=o[3].view(torch.int32), out=o[:32])]
+    wide = torch.randn(40, 160).to(dev)
+    wide[:32, 64] = xs
+    wide[1, 64:96] = ws
+    keep = wide.clone()
+
+    def beside():
+        """out in the first columns; residual, scale, bias and gate in others of the same rows."""
+        got = ops.linear_fp8(xq, wide[:32, 64], wq, ws, wide[2, 96:128], residual=wide[:32, 32:64], gate=wide[3:5, 128:],
+                             rows_per_batch=16, out=wide[:32, :32])
+        assert torch.equal(wide[:, 32:], keep[:, 32:]) and torch.equal(wide[32:], keep[32:])
+        gate = keep[3:5, 128:].repeat_interleave(16, 0)
+        oracle.check_linear(got, *oracle.linear(xq, keep[:32, 64], wq, ws, keep[2, 96:128], residual=keep[:32, 32:64],
+                                                gate_rows=gate))
+    return refused, beside
+
+
+@pytest.mark.parametrize("case", range(7))
+def test_linear_fp8_out_on_parameters(case):
+    with pytest.raises(ValueError):
+        linear_outputs_on_parameters("cpu")[0][case]()
+
+
+def test_linear_fp8_parameters_beside_out():
+    linear_outputs_on_parameters("cpu")[1]()

@@ -153,3 +153,14 @@ def test_in_place_through_another_storage():
     want = r.clone()
     got = ops.rms_norm_quant(x, residual=r, residual_out=cpu.other_storage(r))
     oracle.check_norm_quant((got[0], got[1], r), x, None, want, 1e-6)
+
+
+@pytest.mark.parametrize("case", range(7))
+def test_linear_fp8_out_on_parameters(case):
+    with pytest.raises(ValueError):
+        cpu.linear_outputs_on_parameters(_dev())[0][case]()
+
+
+def test_linear_fp8_parameters_beside_out():
+    cpu.linear_outputs_on_parameters(_dev())[1]()
+    ops.check_status(_dev())
