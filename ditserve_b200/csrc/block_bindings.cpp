@@ -265,8 +265,13 @@ PyObject* rms_norm_quant(PyObject* const* args) {
   if (scale_out.has_value() && (scale_out->sizes() != x.sizes().slice(0, x.dim() - 1) || !scale_out->is_contiguous() ||
                                 scale_out->scalar_type() != at::kFloat || scale_out->device() != dev))
     return nothing();
-  // the row's codes and scale leave while other rows are still read
+  // the row's codes, scale and sum leave while other rows, and the weight, are still read
   const Rows rs{1, rx.rows, rx.rows};
+  if (weight.has_value() && rx.rows > 0 &&
+      ((out.has_value() && !apart_from_vector(*out, rq, *weight, rx.cols)) ||
+       (scale_out.has_value() && !apart_from_vector(*scale_out, rs, *weight, rx.cols)) ||
+       (residual_out.has_value() && !apart_from_vector(*residual_out, rh, *weight, rx.cols))))
+    return nothing();
   auto clear_of = [&](const at::Tensor& t, const Rows& r) {
     return (!out.has_value() || apart(*out, rq, t, r)) && (!scale_out.has_value() || apart(*scale_out, rs, t, r));
   };

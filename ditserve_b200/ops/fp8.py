@@ -100,6 +100,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, *, resid
     outs = [t for t in (out, scale_out, residual_out) if t is not None]
     if any(shares_memory(a, b) for i, a in enumerate(outs) for b in outs[i + 1:]):
         raise ValueError("out, scale_out and residual_out must not share memory")
+    if weight is not None and any(t is not None and shares_memory(t, weight) for t in (out, residual_out)):
+        raise ValueError("out and residual_out must not share memory with weight")
     if not use_kernels(x, weight, residual, out, scale_out, residual_out):
         q, s, h = rms_norm_quant_reference(x, weight, residual, eps)
         q = q if out is None else out.copy_(q)

@@ -185,3 +185,37 @@ def test_linear_fp8_out_on_parameters(case):
 
 def test_linear_fp8_parameters_beside_out():
     linear_outputs_on_parameters("cpu")[1]()
+
+
+def norm_outputs_on_weight(dev):
+    """(calls whose out or residual_out lies on the weight; calls that are right: a scale on the weight, which is
+    written last, and a weight beside the rows of residual_out)"""
+    x, r = torch.randn(8, 64).to(dev, BF), torch.randn(8, 64).to(dev, BF)
+    buf = torch.ones(10, 64, dtype=BF, device=dev)
+    codes = torch.zeros(10, 128, dtype=torch.uint8, device=dev)
+    codes.view(BF).fill_(1.0)
+    refused = [lambda: ops.rms_norm_quant(x, buf[3], residual=r, residual_out=buf[:8]),
+               lambda: ops.rms_norm_quant(x, buf[7], residual=r, residual_out=buf[:8]),
+               lambda: ops.rms_norm_quant(x, codes.view(BF)[2], out=codes.view(E4M3)[:8, 64:])]
+
+    def scale_on_weight():
+        w = (1 + 0.2 * torch.randn(64)).to(dev, BF)
+        before = w.clone()
+        oracle.check_norm_quant(ops.rms_norm_quant(x, w, scale_out=w[16:32].view(FL)), x, before, None, 1e-6)
+
+    def beside():
+        wide = torch.randn(8, 136).to(dev, BF)
+        w = wide[2, 72:]
+        oracle.check_norm_quant(ops.rms_norm_quant(x, w, residual=r, residual_out=wide[:, :64]), x, w, r, 1e-6)
+    return refused, (scale_on_weight, beside)
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_rms_norm_quant_outputs_on_weight(case):
+    with pytest.raises(ValueError):
+        norm_outputs_on_weight("cpu")[0][case]()
+
+
+@pytest.mark.parametrize("case", range(2))
+def test_rms_norm_quant_weight_near_outputs(case):
+    norm_outputs_on_weight("cpu")[1][case]()

@@ -164,3 +164,14 @@ def test_linear_fp8_out_on_parameters(case):
 def test_linear_fp8_parameters_beside_out():
     cpu.linear_outputs_on_parameters(_dev())[1]()
     ops.check_status(_dev())
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_rms_norm_quant_outputs_on_weight(case):
+    with pytest.raises(ValueError):
+        cpu.norm_outputs_on_weight(_dev())[0][case]()
+
+
+@pytest.mark.parametrize("case", range(2))
+def test_rms_norm_quant_weight_near_outputs(case):
+    cpu.norm_outputs_on_weight(_dev())[1][case]()
