@@ -479,6 +479,13 @@ PyObject* rope_axes(PyObject* const* args) {
                         (out.has_value() && k_out.has_value() && !apart(*out, to[0], *k_out, to[1]))))
     return nothing();
   const int64_t rows = in[0].rows;
+  // positions are read while rows leave
+  if (rows > 0 && pos.numel() > 0) {
+    const bool packed = pos.dim() == 1 || pos_axes == 1 || pos.stride(1) == 1;
+    const Rows rp{pos.stride(0) == 0 ? 1 : pos.size(0), pos_axes, pos.stride(0)};
+    for (int i = 0; i < 2; ++i)
+      if (o[i].has_value() && (packed ? !apart(*o[i], to[i], pos, rp) : spans_meet(*o[i], pos))) return nothing();
+  }
   if (rows > 0 && (pos.size(0) == 0 || rows % pos.size(0) != 0)) return nothing();
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor y[2];

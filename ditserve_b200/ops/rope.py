@@ -11,6 +11,7 @@ import functools
 import torch
 
 from ._ext import ext, launch, use_kernels
+from ._memory import shares_memory
 from .fp8 import _partial_overlap, _rows_view
 
 _POSITIONS = (torch.int64, torch.int32, torch.float32, torch.float64)
@@ -56,7 +57,8 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
     head_dim together; elements behind them pass through.  Pair j of an axis of d elements turns by
     position * theta^(-2j / d); theta is one number or one for each axis.  layout "interleaved" pairs
     elements (2i, 2i + 1), "half" pairs (i, i + sum(dims) / 2).  inverse turns the other way.  x and k
-    (bf16, fp16 or fp32) may differ in heads.  out / k_out may be x / k themselves."""
+    (bf16, fp16 or fp32) may differ in heads.  out / k_out may be x / k themselves; they share no memory with
+    what else is read or written (columns of one buffer are apart)."""
     if x.is_cuda and layout in ("interleaved", "half"):
         # by value: a tensor among them would be told apart by its identity
         plan = _plan(tuple(map(int, dims)),
@@ -96,6 +98,8 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
             raise ValueError("k must be [..., heads * head_dim] with x's tokens and type")
         if k_out is not None and (k_out.shape != k.shape or k_out.dtype != k.dtype):
             raise ValueError("k_out must have k's shape and type")
+    if any(o is not None and shares_memory(o, positions) for o in (out, k_out)):
+        raise ValueError("out and k_out must not share memory with positions")
     if not use_kernels(x, positions, k, out, k_out):
         got = []
         for t, o in ((x, out), (k, k_out)):

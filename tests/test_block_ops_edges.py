@@ -219,3 +219,31 @@ def test_rms_norm_quant_outputs_on_weight(case):
 @pytest.mark.parametrize("case", range(2))
 def test_rms_norm_quant_weight_near_outputs(case):
     norm_outputs_on_weight("cpu")[1][case]()
+
+
+def rope_outputs_on_positions(dev):
+    """(calls whose outputs lie on the positions; positions in columns beside the rows of out)"""
+    pos = torch.zeros(8, 64, dtype=torch.int64, device=dev)
+    x = torch.randn(8, 128).to(dev)
+    refused = [lambda: ops.rope_axes(x, pos[3, :8], (64,), out=pos.view(FL)),
+               lambda: ops.rope_axes(x, pos[:, :3], (44, 42, 42), out=pos.view(FL)),
+               lambda: ops.rope_axes(x, pos.t()[:8, :3], (44, 42, 42), k=x, k_out=pos.view(FL))]
+
+    def beside():
+        wide = torch.zeros(8, 136, device=dev)
+        p = wide[:, 130:133]
+        p.copy_(torch.arange(24).view(8, 3))
+        want = p.clone()
+        oracle.check_rope(ops.rope_axes(x, p, (44, 42, 42), out=wide[:, :128]), x, want, (44, 42, 42), 128, (1e4,) * 3)
+        assert torch.equal(p, want)
+    return refused, beside
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_rope_axes_outputs_on_positions(case):
+    with pytest.raises(ValueError):
+        rope_outputs_on_positions("cpu")[0][case]()
+
+
+def test_rope_axes_positions_beside_out():
+    rope_outputs_on_positions("cpu")[1]()

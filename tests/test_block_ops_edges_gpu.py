@@ -175,3 +175,13 @@ def test_rms_norm_quant_outputs_on_weight(case):
 @pytest.mark.parametrize("case", range(2))
 def test_rms_norm_quant_weight_near_outputs(case):
     cpu.norm_outputs_on_weight(_dev())[1][case]()
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_rope_axes_outputs_on_positions(case):
+    with pytest.raises(ValueError):
+        cpu.rope_outputs_on_positions(_dev())[0][case]()
+
+
+def test_rope_axes_positions_beside_out():
+    cpu.rope_outputs_on_positions(_dev())[1]()
