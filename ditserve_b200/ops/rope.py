@@ -98,15 +98,15 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, dims, *, k: torch.Tensor
             raise ValueError("k must be [..., heads * head_dim] with x's tokens and type")
         if k_out is not None and (k_out.shape != k.shape or k_out.dtype != k.dtype):
             raise ValueError("k_out must have k's shape and type")
+    if out is not None and k_out is not None and shares_memory(out, k_out):
+        raise ValueError("the outputs of x and k must be apart")
     if any(o is not None and shares_memory(o, positions) for o in (out, k_out)):
         raise ValueError("out and k_out must not share memory with positions")
     if not use_kernels(x, positions, k, out, k_out):
-        got = []
-        for t, o in ((x, out), (k, k_out)):
-            if t is not None:
-                r = rope_axes_reference(t.reshape(-1, t.shape[-1]), positions, dims, head_dim, theta, layout,
-                                        inverse).reshape(t.shape)
-                got.append(r if o is None else o.copy_(r))
+        # both are rotated before either is stored: out may lie on k
+        got = [rope_axes_reference(t.reshape(-1, t.shape[-1]), positions, dims, head_dim, theta, layout, inverse)
+               .reshape(t.shape) for t in (x, k) if t is not None]
+        got = [r if o is None else o.copy_(r) for r, o in zip(got, (out, k_out))]
         return got[0] if k is None else tuple(got)
     # what the kernel does not take as it is: columns apart, several outputs to tell apart
     t2, o2, w = [], [], [x.shape[-1], 0 if k is None else k.shape[-1]]

@@ -247,3 +247,17 @@ def test_rope_axes_outputs_on_positions(case):
 
 def test_rope_axes_positions_beside_out():
     rope_outputs_on_positions("cpu")[1]()
+
+
+def test_rope_axes_out_on_k():
+    """On the CPU x' may go where k was: k' is of the k that came in.  x' and k' in one place are refused."""
+    x, k = torch.randn(6, 64), torch.randn(6, 64)
+    pos, was = torch.arange(6), k.clone()
+    y, ky = ops.rope_axes(x, pos, (64,), k=k, head_dim=64, out=k)
+    assert y is k
+    oracle.check_rope(y, x, pos[:, None], (64,), 64, (1e4,))
+    oracle.check_rope(ky, was, pos[:, None], (64,), 64, (1e4,))
+    o = torch.zeros(7, 64)
+    for a, b in ((o[:6], o[:6]), (o[:6], o[1:])):
+        with pytest.raises(ValueError):
+            ops.rope_axes(x, pos, (64,), k=was, head_dim=64, out=a, k_out=b)
