@@ -18,6 +18,7 @@
 #include <cfloat>
 #include <cmath>
 #include <mutex>
+#include <numeric>
 
 #include "kernels.h"
 
@@ -189,9 +190,10 @@ bool apart(const at::Tensor& out, const Rows& o, const at::Tensor& in, const Row
   const int64_t lo = reinterpret_cast<int64_t>(out.data_ptr()), at = reinterpret_cast<int64_t>(in.data_ptr());
   const int64_t hi = lo + ((o.rows - 1) * o.stride + o.cols) * eo, end = at + ((i.rows - 1) * i.stride + i.cols) * ei;
   if (hi <= at || end <= lo) return true;
-  // a single row counts as one of the other's
-  const int64_t pitch = o.rows > 1 ? o.stride * eo : i.stride * ei;
-  if (pitch <= 0 || (o.rows > 1 && i.rows > 1 && i.stride * ei != pitch) || (o.rows == 1 && i.rows == 1)) return false;
+  // all rows of either start in one place of this pitch; a single row in one of any
+  if ((o.rows > 1 && o.stride <= 0) || (i.rows > 1 && i.stride <= 0)) return false;
+  const int64_t pitch = std::gcd(o.rows > 1 ? o.stride * eo : 0, i.rows > 1 ? i.stride * ei : 0);
+  if (pitch == 0) return false;
   const int64_t d = ((lo - at) % pitch + pitch) % pitch;
   return d >= i.cols * ei && d + o.cols * eo <= pitch;
 }
@@ -557,6 +559,10 @@ PyObject* cross_attention(PyObject* const* args) {
     a.mask_row = m.stride(0);
     a.mask_col = m.stride(1);
   }
+  // lengths and mask are read while outputs leave
+  if (out.has_value() && ((kv_lens.has_value() && spans_meet(*out, *kv_lens)) ||
+                          (key_mask.has_value() && spans_meet(*out, *key_mask))))
+    return nothing();
   const double s = args[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : float_arg(args[7]);
   // the kernels multiply scores, -inf among them, by scale * log2(e) in fp32: neither zero nor infinite there
   if (!(s >= FLT_TRUE_MIN) || !(s * M_LOG2E <= FLT_MAX)) return nothing();

@@ -1,6 +1,8 @@
 """Whether tensors share bytes, for the checks of outputs against what a call reads or writes besides."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 
@@ -33,8 +35,8 @@ def shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     b0, b1, run_b, n_b, pitch_b = _runs(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    pitch_a, pitch_b = (pitch_b if n_a == 1 else pitch_a), (pitch_a if n_b == 1 else pitch_b)
-    if pitch_a != pitch_b or not pitch_a:
+    pitch = math.gcd(pitch_a, pitch_b)  # all runs of either start in one place of it
+    if not pitch:
         return True
-    d = (a0 - b0) % pitch_a
-    return d < run_b or d + run_a > pitch_a
+    d = (a0 - b0) % pitch
+    return d < run_b or d + run_a > pitch

@@ -12,6 +12,7 @@ import math
 import torch
 
 from ._ext import launch, status_word, use_kernels
+from ._memory import shares_memory
 
 # fp32's smallest number; its largest over log2(e), which the exponentials' base takes in
 SCALE_MIN, SCALE_MAX = 2.0 ** -149, torch.finfo(torch.float32).max / math.log2(math.e)
@@ -107,6 +108,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         raise ValueError("out must have q's shape and type")
     if out is not None and any(_shares_memory(out, t) for t in (q, k, v)):
         raise ValueError("out must not share memory with q, k or v")
+    if out is not None and any(t is not None and shares_memory(out, t) for t in (kv_lens, key_mask)):
+        raise ValueError("out must not share memory with kv_lens or key_mask")
     if not use_kernels(q, k, v, kv_lens, key_mask, out):
         o, lse = cross_attention_reference(q, k, v, heads, heads_kv, kv_lens, key_mask, scale, True)
         o = o if out is None else out.copy_(o)
@@ -119,6 +122,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     status_word(q.device)
     if kv_lens is not None:
         kv_lens = kv_lens.clamp(0, Sk).to(torch.int32).contiguous()
+    if out is not None and key_mask is not None and _shares_memory(out, key_mask):
+        key_mask = key_mask.clone()  # beside out's rows
     got = launch("cross_attention", _strided(q), _strided(k), _strided(v), heads, heads_kv, kv_lens, key_mask, scale, out,
                  return_lse)
     if got is None:

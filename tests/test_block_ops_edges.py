@@ -261,3 +261,36 @@ def test_rope_axes_out_on_k():
     for a, b in ((o[:6], o[:6]), (o[:6], o[1:])):
         with pytest.raises(ValueError):
             ops.rope_axes(x, pos, (64,), k=was, head_dim=64, out=a, k_out=b)
+
+
+def cross_outputs_on_masks(dev, sq):
+    """(calls whose out lies on the lengths or the mask; lengths and mask in columns beside out's rows)"""
+    q, k = torch.randn(2, sq, 128).to(dev, BF), torch.randn(2, 9, 128).to(dev, BF)
+    out = torch.zeros(2, sq, 128, dtype=BF, device=dev)
+    flat = out.view(-1)
+    refused = [lambda: ops.cross_attention(q, k, k, 2, kv_lens=flat.view(torch.int32)[:2], out=out),
+               lambda: ops.cross_attention(q, k, k, 2, kv_lens=flat[-8:].view(torch.int64), out=out),
+               lambda: ops.cross_attention(q, k, k, 2, key_mask=flat.view(torch.bool)[64:82].view(2, 9), out=out)]
+
+    def beside():
+        wide = torch.zeros(2, sq, 160, dtype=BF, device=dev)
+        lens = wide[:, 0, 128:130].view(torch.int32)[:, 0]
+        lens.copy_(torch.tensor([9, 4]))
+        mask = wide[:, 0, 132:141].view(torch.bool)[:, :9]
+        mask.copy_(torch.tensor([[1, 1, 0, 1, 0, 1, 1, 1, 1], [0, 1, 1, 1, 1, 1, 1, 1, 1]]).bool())
+        allowed = mask & (torch.arange(9, device=dev) < lens[:, None])
+        keep = wide.clone()
+        o = ops.cross_attention(q, k, k, 2, kv_lens=lens, key_mask=mask, out=wide[..., :128])
+        oracle.check_cross(o, None, q, k, k, 2, allowed=allowed)
+        assert torch.equal(wide[..., 128:], keep[..., 128:])
+    return refused, beside
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_cross_attention_out_on_masks(case):
+    with pytest.raises(ValueError):
+        cross_outputs_on_masks("cpu", 4)[0][case]()
+
+
+def test_cross_attention_masks_beside_out():
+    cross_outputs_on_masks("cpu", 4)[1]()

@@ -185,3 +185,15 @@ def test_rope_axes_outputs_on_positions(case):
 
 def test_rope_axes_positions_beside_out():
     cpu.rope_outputs_on_positions(_dev())[1]()
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_cross_attention_out_on_masks(case):
+    with pytest.raises(ValueError):
+        cpu.cross_outputs_on_masks(_dev(), 4)[0][case]()
+
+
+@pytest.mark.parametrize("sq", [4, 300])
+def test_cross_attention_masks_beside_out(sq):
+    cpu.cross_outputs_on_masks(_dev(), sq)[1]()
+    ops.check_status(_dev())
