@@ -539,7 +539,10 @@ PyObject* cross_attention(PyObject* const* args) {
         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
       return false;
     if (rows > 1 && t.stride(1) < (output ? cols : 8)) return false;
-    return !output || B == 1 || t.stride(0) >= cols;
+    if (!output || B == 1) return true;
+    // an output's entries lie behind one another, or between one another's rows
+    const int64_t entry = (rows - 1) * t.stride(1) + cols, row = (B - 1) * t.stride(0) + cols;
+    return t.stride(0) >= entry || (t.stride(0) >= cols && (rows == 1 || t.stride(1) >= row));
   };
   if (!fits(q, Sq, width, false) || !fits(k, Sk, heads_kv * d, false) || !fits(v, Sk, heads_kv * d, false)) return nothing();
   if (out.has_value()) {

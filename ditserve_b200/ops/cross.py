@@ -52,6 +52,16 @@ def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _meets_itself(t: torch.Tensor) -> bool:
+    """Whether elements of ``t`` may lie on one another: axes that are not nested in one another count as that."""
+    extent = 1
+    for stride, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if stride < extent:
+            return True
+        extent += stride * (n - 1)
+    return False
+
+
 def _strided(t: torch.Tensor) -> torch.Tensor:
     ok = t.stride(2) == 1 and t.stride(1) % 8 == 0 and (t.stride(1) > 0 or t.shape[1] == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
@@ -106,6 +116,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         raise ValueError("scale must be positive and finite in fp32, and so must scale * log2(e)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise ValueError("out must have q's shape and type")
+    if out is not None and out.numel() and _meets_itself(out):
+        raise ValueError("out must have batch entries and rows apart")
     if out is not None and any(_shares_memory(out, t) for t in (q, k, v)):
         raise ValueError("out must not share memory with q, k or v")
     if out is not None and any(t is not None and shares_memory(out, t) for t in (kv_lens, key_mask)):

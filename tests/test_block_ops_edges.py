@@ -294,3 +294,28 @@ def test_cross_attention_out_on_masks(case):
 
 def test_cross_attention_masks_beside_out():
     cross_outputs_on_masks("cpu", 4)[1]()
+
+
+def cross_out_layouts(dev, sq):
+    """(strides of out whose entries or rows meet; strides whose do not: entries behind or between one another)"""
+    q, k = torch.randn(3, sq, 128).to(dev, BF), torch.randn(3, 9, 128).to(dev, BF)
+    flat = torch.full((3 * 2 * sq * 256,), 7.0, dtype=BF, device=dev)
+
+    def call(strides):
+        out = flat.as_strided((3, sq, 128), (*strides, 1))
+        o = ops.cross_attention(q, k, k, 2, out=out)
+        oracle.check_cross(o, None, q, k, k, 2)
+        mark = torch.zeros_like(flat, dtype=torch.bool)
+        mark.as_strided((3, sq, 128), (*strides, 1)).fill_(True)
+        assert (flat[~mark] == 7).all()
+    refused = [(128, 128), (128 * (sq - 1), 128), (256, 128), (128, 256), (0, 128)]
+    taken = [(128 * sq, 128), (256 * sq + 8, 256), (128, 3 * 128), (136, 3 * 136), (256, 3 * 256 - 128)]
+    return refused, taken, call
+
+
+@pytest.mark.parametrize("case", range(5))
+def test_cross_attention_out_entries_apart(case):
+    refused, taken, call = cross_out_layouts("cpu", 4)
+    with pytest.raises(ValueError):
+        call(refused[case])
+    call(taken[case])

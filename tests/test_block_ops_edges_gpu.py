@@ -197,3 +197,24 @@ def test_cross_attention_out_on_masks(case):
 def test_cross_attention_masks_beside_out(sq):
     cpu.cross_outputs_on_masks(_dev(), sq)[1]()
     ops.check_status(_dev())
+
+
+@pytest.mark.parametrize("sq", [4, 300])
+@pytest.mark.parametrize("case", range(5))
+def test_cross_attention_out_entries_apart(case, sq):
+    refused, taken, call = cpu.cross_out_layouts(_dev(), sq)
+    with pytest.raises(ValueError):
+        call(refused[case])
+    call(taken[case])
+    ops.check_status(_dev())
+
+
+def test_cross_attention_tiles_between_rows():
+    """[S, B, width] buffers: entries between one another's rows, through tile loads and stores."""
+    q, k, v = (_randn(n, 3, 24 * 64 + 8, seed=s, dtype=BF)[..., 8:].transpose(0, 1) for n, s in ((520, 1), (300, 2), (300, 3)))
+    out = torch.full((521, 3, 24 * 64 + 8), 7.0, device=_dev(), dtype=BF)
+    ops.cross_attention(q, k, v, 24, out=out[:520, :, :24 * 64].transpose(0, 1))
+    ops.check_status(_dev())
+    want = ops.cross_attention(q.contiguous(), k.contiguous(), v.contiguous(), 24)
+    assert torch.equal(out[:520, :, :24 * 64].transpose(0, 1), want)
+    assert (out[520] == 7).all() and (out[..., 24 * 64:] == 7).all()
