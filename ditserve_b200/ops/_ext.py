@@ -62,13 +62,15 @@ class KernelTimer:
         _timer = self._prev
         return False
 
-    def wrap(self, name: str, fn):
+    def wrap(self, name: str, fn, skip_none: bool = False):
+        """``fn`` timed as ``name``; with ``skip_none`` a call that returns None launched nothing and leaves no record."""
         def timed(*args, **kwargs):
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             e0.record()
             out = fn(*args, **kwargs)
             e1.record()
-            self.records.append((name, e0, e1))
+            if not skip_none or out is not None:
+                self.records.append((name, e0, e1))
             return out
         return timed
 
@@ -95,7 +97,7 @@ def launch(name: str, *args):
     arguments need another layout or are wrong; counts (and times) the launch otherwise."""
     fn = getattr(_ext or ext(), name)
     if _timer is not None:
-        fn = _timer.wrap(name, fn)
+        fn = _timer.wrap(name, fn, skip_none=True)
     got = fn(*args)
     if got is not None:
         _launches[name] = _launches.get(name, 0) + 1

@@ -319,3 +319,24 @@ def test_cross_attention_out_entries_apart(case):
     with pytest.raises(ValueError):
         call(refused[case])
     call(taken[case])
+
+
+def test_timer_records_launches_alone(monkeypatch):
+    """An entry that returns None launched nothing: no record and no count, whatever is timed."""
+    from ditserve_b200.ops import _ext
+
+    class Event:
+        def __init__(self, enable_timing):
+            pass
+
+        def record(self):
+            pass
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    answers = iter([None, "out"])
+    fake = type("Ext", (), {"op": staticmethod(lambda *a: next(answers)), "other": staticmethod(lambda: None)})
+    monkeypatch.setattr(_ext, "_ext", fake)
+    monkeypatch.setattr(_ext, "_launches", {})
+    with ops.KernelTimer() as timer:
+        assert _ext.launch("op", 1) is None and _ext.launch("op", 1) == "out"
+        assert _ext.kernel("other")() is None  # entries that return nothing always launch
+    assert [r[0] for r in timer.records] == ["op", "other"] and ops.launch_counts() == {"op": 1, "other": 1}
