@@ -9,6 +9,7 @@
 // the binding library took 1.5 us, a quarter of a small call.
 #include <torch/extension.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -94,10 +95,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     e.restore();
   } catch (const BadArgument& e) {
     PyErr_SetString(PyExc_TypeError, e.what());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  } catch (...) {
-    PyErr_SetString(PyExc_RuntimeError, "unknown error");
+  } catch (...) {  // torch's own classes: torch.OutOfMemoryError among them
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

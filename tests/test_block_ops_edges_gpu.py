@@ -218,3 +218,28 @@ def test_cross_attention_tiles_between_rows():
     want = ops.cross_attention(q.contiguous(), k.contiguous(), v.contiguous(), 24)
     assert torch.equal(out[:520, :, :24 * 64].transpose(0, 1), want)
     assert (out[520] == 7).all() and (out[..., 24 * 64:] == 7).all()
+
+
+# ---- errors -----------------------------------------------------------------------------------
+def test_out_of_memory_is_torchs_error():
+    """An allocation beyond the allocator's limit (a limit of this process, not the device's end): torch's own class."""
+    x = torch.zeros(1, 64, device=_dev(), dtype=BF).expand(1 << 22, 64)  # 256 MB of codes
+    xq, xs = ops.quantize_rows_fp8(torch.zeros(16, 64, device=_dev()))
+    wq, ws = ops.empty_fp8(1 << 22, 64, _dev()), torch.ones(1 << 22, device=_dev())
+    q = torch.zeros(1, 1, 128, device=_dev(), dtype=BF).expand(1, 1 << 20, 128)
+    calls = [lambda: ops.rms_norm_quant(x), lambda: ops.linear_fp8(xq, xs, wq, ws),
+             lambda: ops.rope_axes(x, torch.zeros(1, 1, device=_dev()), (64,), head_dim=64),
+             lambda: ops.cross_attention(q, q[:, :3], q[:, :3], 2)]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (32 << 20)) /
+                                                   torch.cuda.get_device_properties(0).total_memory)
+        for call in calls:
+            with pytest.raises(torch.cuda.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert ops.rms_norm_quant(x[:4])[0].shape == (4, 64)
+    with pytest.raises(TypeError):
+        ops._ext.launch("rms_norm_quant", 1, None, None, 1e-6, None, None, None)
