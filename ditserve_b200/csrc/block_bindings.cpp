@@ -332,7 +332,8 @@ PyObject* linear_fp8(PyObject* const* args) {
   if (a.status == nullptr || !fp8_rows(x, dev, rx) || w.dim() != 2 || !fp8_rows(w, dev, rw) || rw.cols != rx.cols)
     return nothing();
   const int64_t M = rx.rows, K = rx.cols, N = rw.rows;
-  if (M > (1 << 30) || N > (1 << 30)) return nothing();
+  // a tile's products over more values would outlast the kernels' wait for them (2^28: 0.8 s of 2)
+  if (M > (1 << 30) || N > (1 << 30) || K > (1 << 28)) return nothing();
   if (sx.sizes() != x.sizes().slice(0, x.dim() - 1) || sx.scalar_type() != at::kFloat || sx.device() != dev ||
       !sx.is_contiguous() || !is_vector(sw, dev, N, at::kFloat))
     return nothing();

@@ -162,7 +162,7 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     """y = epilogue(x_scale[m] * w_scale[n] * sum_k xq[m, k] wq[n, k] + b[n]), epilogues as in ``linear``.
 
     xq: float8_e4m3fn [..., K] with fp32 x_scale [...]; wq float8_e4m3fn [N, K] with fp32 w_scale [N]
-    (``quantize_rows_fp8``).  Any M, N and K; rows that do not start on 16 bytes (K not a multiple
+    (``quantize_rows_fp8``).  Any M and N up to 2^30, K up to 2^28; rows that do not start on 16 bytes (K not a multiple
     of 16 in a packed matrix) are copied first on every call, which ``empty_fp8`` avoids.  The result, b and residual share
     ``out_dtype`` (bf16, fp16 or fp32; ``out`` decides if given).  ``out`` may be ``residual`` itself, but shares no memory
     with what else is read (columns of one buffer are apart).
@@ -178,6 +178,8 @@ def linear_fp8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scal
     if xq.dim() < 1 or wq.dim() != 2 or xq.shape[-1] != wq.shape[1] or wq.shape[1] == 0:
         raise ValueError("xq [..., K] and wq [N, K] must share K >= 1")
     lead, K, N = xq.shape[:-1], wq.shape[1], wq.shape[0]
+    if K > 1 << 28 or N > 1 << 30 or xq.numel() // K > 1 << 30:
+        raise ValueError("linear_fp8 takes up to 2^28 values and 2^30 rows and channels")
     if x_scale.dtype != torch.float32 or x_scale.shape != lead:
         raise ValueError("x_scale must be fp32 of xq's shape without its last axis")
     if w_scale.dtype != torch.float32 or w_scale.shape != (N,):

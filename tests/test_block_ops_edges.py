@@ -340,3 +340,11 @@ def test_timer_records_launches_alone(monkeypatch):
         assert _ext.launch("op", 1) is None and _ext.launch("op", 1) == "out"
         assert _ext.kernel("other")() is None  # entries that return nothing always launch
     assert [r[0] for r in timer.records] == ["op", "other"] and ops.launch_counts() == {"op": 1, "other": 1}
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 2, (1 << 28) + 16), ((1 << 30) + 1, 1, 1), (1, (1 << 30) + 1, 1)])
+def test_linear_fp8_refuses_sizes(m, n, k, dev="cpu"):
+    """Broadcast operands: refused by their sizes, before anything of them is laid out."""
+    one, s = torch.zeros(1, 1, device=dev).to(E4M3), torch.ones(1, device=dev)
+    with pytest.raises(ValueError, match="up to"):
+        ops.linear_fp8(one.expand(m, k), s.expand(m), one.expand(n, k), s.expand(n))

@@ -243,3 +243,8 @@ def test_out_of_memory_is_torchs_error():
     assert ops.rms_norm_quant(x[:4])[0].shape == (4, 64)
     with pytest.raises(TypeError):
         ops._ext.launch("rms_norm_quant", 1, None, None, 1e-6, None, None, None)
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 2, (1 << 28) + 16), ((1 << 30) + 1, 1, 1), (1, (1 << 30) + 1, 1)])
+def test_linear_fp8_refuses_sizes(m, n, k):
+    cpu.test_linear_fp8_refuses_sizes(m, n, k, _dev())
