@@ -3,9 +3,12 @@
 //   o[b, i, h] = sum_j p_ij v[b, j, hk] / sum_j p_ij,  p_ij = exp(scale q_i k_j - max_j), j over the keys of
 //   batch entry b that its valid length and its key mask leave; nothing left: o = 0 and lse = -inf.
 //
-// Scores, the running maximum and sum and the output's sums are fp32; p is rounded to the values'
-// type for the second product, as its operand has to be.  Keys that are masked never reach a product
-// with their value: their v is replaced by zero, so that NaN or infinities in padding do no harm.
+// Scores, the running maximum and sum (Milakov and Gimelshein, "Online normalizer calculation for softmax", 2018) and the
+// output's sums are fp32.  p is rounded to the values' type for the second product, whose operands have 16 bits: half
+// a step of each weight, while the sum below keeps 32 bits.  Against 64 bits the output errs 1.2 to 1.4 times as much as
+// with weights of 32 bits (bf16 0.0023 of it for 0.0017, fp16 0.00028 for 0.00021), and fp16 weights below 2^-25 of the
+// largest count in the sum alone.  Keys that are masked never reach a product with their value: their v is replaced by
+// zero, so that NaN or infinities in padding do no harm.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -302,16 +305,20 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 //   warp 2        puts zeros in the values of masked keys (only with lengths or a mask)
 //   warps 4..7    softmax and output of tile A, a row a thread; warps 8..11 of tile B
 // TMEM: S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B [384, 384 + D).  P is written over the first
-// half of its S as the second product's TMEM operand, in two chunks of 64 keys.  O is rescaled only when the
-// running maximum has grown by more than 2^8; P then is at most 256 and exact sums hold in fp32.
+// half of its S as the second product's TMEM operand, in two chunks of 64 keys.  The maximum that is
+// subtracted may lag, since a common factor cancels in the quotient (a known variant): O is rescaled only when it has
+// grown by more than 2^8; P then is at most 256, which both types hold.
 // Bound by the chain softmax (2000 cycles a step), P to PV, PV, next S (1400) of a tile, which two tiles in turn cover to
 // about 60 % of the tensor pipe's time, and at a unit's end by its output (2500).  32760 queries of 12 heads over 4096
-// keys take 690 us (1190 TFLOP/s), 2 x 32760 over 512 keys 205 us (1000).  Measured and not kept: P through shared memory
+// keys take 690 to 765 us from box to box (1190 to 1080 TFLOP/s), 2 x 32760 over 512 keys 207 to 220 (1000 to 940).
+// Measured and not kept (against the form of the day, measured alike): P through shared memory
 // with the next scores formed during the exponentials (268 us against 240 at 4096 x 4096: operands, P and loads together
 // exceed the shared memory's rate), two threads a row (213 against 197), output warps of their own, every fourth pair of
 // exponentials as a polynomial (238 against 197), a product warp a tile (218 against 197), key tiles of 64 with the scores
 // formed two ahead (266 against 218; with a product warp a tile 256): a barrier's wait takes 200 cycles behind the other
-// tile's exponentials in the queue, and smaller tiles wait twice as often.
+// tile's exponentials in the queue, and smaller tiles wait twice as often.  A ragged last key tile costs what a full one
+// does, and units of one key head's rows are not split over keys where they leave SMs without one: 4 x 288 queries over
+// 764 keys of 12 heads of 64 take 15.6 us (floor 2.0), 2 x 845 over 1654 of 24 heads 53 (10.9).
 constexpr int kQT = 128, kKT = 128, kPChunks = 2;
 constexpr int kTileThreads = 384;
 

@@ -593,8 +593,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // 0.1 us * bn / 256 (8960 x 1536 channels at 32760 rows: 0.39, 0.355 and 0.325 us for 256, 192 and 128
 // channels), bound by the L2's traffic into shared memory more than by the products, so few wide rounds
 // beat many narrow ones, and a single round takes the narrowest tile that keeps it one.  32760 rows to 8960 channels from
-// 1536 values take 316 us as a single launch (0.90 of the measured 8-bit rate), 365 to 450 in a row of them under the
-// power limit.
+// 1536 values take 311 to 322 us as a single launch without an activation, 339 to 351 with GELU (0.88 and 0.81 of twice
+// the measured 16-bit rate; the 8-bit rate itself is not measured), 365 to 450 in a row of them under the power limit.
+// The cost knows no epilogue: where K is short it is the time (474 rows to 6656 channels from 64 values with a gated
+// residual 9.4 us).
 // `unit` (16 or 32) keeps whole 64-byte units of the output in a tile, which is how the epilogue goes through it.
 // More tiles than CTAs, but fewer than twice as many: twins bring them into one round, and a k-block of x then serves
 // both (the tiles' outputs leave behind one another, which a second round would not spare either): 512 rows to 10240
@@ -675,7 +677,9 @@ void launch_tiles(const LinearFp8Args& a, const TilePlan& plan, cudaStream_t s) 
 // 10240 channels and values; up to 16 rows the first form always):
 //   rows    2 (3.5 with K split over blocks) + the operands' bytes out of L2, 16 + 8 kM rows a block, at 4.8 TB/s
 //   tiles   3.2 + rounds * (k-blocks * (0.24 + 0.1 bn / 256) + 0.6)
-// e.g. 32 rows to 1024 channels from 4096 values 6.4 and 11.3, to 9216 from 1536 10.3 and 8.2.
+// e.g. 32 rows to 1024 channels from 4096 values 6.4 and 11.3, to 9216 from 1536 10.3 and 8.2.  Neither knows epilogues
+// or warps without a chunk of K, which count where K is short: 100 rows to 4544 channels from 128 values with a
+// residual take 11.1 in the first form, where the rule expects 3.5.
 bool rows_are_faster(const LinearFp8Args& a) {
   if (a.M <= 16 || a.M > 4096) return a.M <= 16;
   const int rows = 32;

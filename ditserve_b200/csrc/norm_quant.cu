@@ -7,13 +7,16 @@
 //
 // The sum over a row, the norm and the scale are fp32.  Two roundings to fewer bits: h, because the
 // next layer reads the same stored stream, and q, which is the output.  A NaN or an infinity in a
-// row makes its scale and all its q NaN (the maximum passes NaN on).
+// row makes its scale and all its q NaN (the maximum passes NaN on).  The factors come in another order than above, h w
+// once for maximum and output, then rstd, then 1 / s: y / s errs by some 2^-22 of itself, so a code whose value lies
+// that close to the border of two steps may be either.
 //
 // One pass over memory: a row stays in registers between its sum of squares, its maximum and its
 // quantisation, so an element costs its own read(s), the stored h and one byte.  Bound by HBM: 32760 x 1536 in bf16
-// with a residual takes 64 us (5.5 TB/s, the rate of a copy of as many bytes); rows that start off 16 bytes go in pieces
-// of 4 bytes (1530 wide: 105 us) or single elements (1531: 148 us).  Measured and not kept: cutting such rows' vectors out
-// of two aligned ones, stores put together across lanes (148 and 158 us).
+// with a residual takes 57 us in a graph (6.2 TB/s), 60 call by call (a copy of as many bytes: 63).  Without a residual
+// instructions bound it, the weights' two conversions a row among them: 35 us (4.3 TB/s).  Rows that start off 16 bytes
+// go in pieces of 4 bytes (1530 wide: 100 us) or single elements (1531: 142 us).  Measured and not kept: cutting such
+// rows' vectors out of two aligned ones, stores put together across lanes (148 and 158 us call by call).
 #include <cuda_fp8.h>
 
 #include "elem.cuh"
