@@ -19,7 +19,8 @@ def test_shares_memory_against_the_bytes():
     views = [buf, buf[:16], buf[16:], buf[8:24].view(FL), buf.view(6, 16)[:, :8], buf.view(6, 16)[:, 8:],
              buf.view(6, 16)[:, 12:].view(FL), buf.view(6, 16)[2:, 4:12], buf.view(6, 16)[1:3], buf.view(2, 3, 16)[..., 4:8],
              buf.view(6, 16)[::2, :8], buf.view(6, 16)[1::2], buf[4:84].view(5, 16)[:, 8:], buf[95:], buf[:0],
-             buf.view(FL).view(6, 4)[:, 3], buf.view(FL)[3::4][:2], buf[:1].expand(7)]
+             buf.view(FL).view(6, 4)[:, 3], buf.view(FL)[3::4][:2], buf[:1].expand(7),
+             buf.view(2, 3, 16)[:, :2, :8], buf.view(2, 3, 16)[:, 1:, 8:], buf.view(2, 3, 16)[:, 2, 4:8]]
     exact = list(range(len(views)))
 
     def touched(v):
@@ -36,7 +37,7 @@ def test_shares_memory_against_the_bytes():
             got = shares_memory(views[i], views[j])
             assert got or not meet, (i, j)
     # the layouts that calls use: exactly
-    for i in (1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 13, 14, 15):
+    for i in (1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 13, 14, 15, 18, 19):
         for j in (1, 2, 4, 5, 6, 9, 13, 14, 15):
             assert shares_memory(views[i], views[j]) == bool((touched(views[i]) & touched(views[j])).any()), (i, j)
 
