@@ -310,7 +310,7 @@ void launch_few(const CrossAttnArgs& a, cudaStream_t s) {
 // grown by more than 2^8; P then is at most 256, which both types hold.
 // Bound by the chain softmax (2000 cycles a step), P to PV, PV, next S (1400) of a tile, which two tiles in turn cover to
 // about 60 % of the tensor pipe's time, and at a unit's end by its output (2500).  32760 queries of 12 heads over 4096
-// keys take 690 to 765 us from box to box (1190 to 1080 TFLOP/s), 2 x 32760 over 512 keys 207 to 220 (1000 to 940).
+// keys take 690 to 765 us from one B200 to another (1190 to 1080 TFLOP/s), 2 x 32760 over 512 keys 207 to 220 (1000 to 940).
 // Measured and not kept (against the form of the day, measured alike): P through shared memory
 // with the next scores formed during the exponentials (268 us against 240 at 4096 x 4096: operands, P and loads together
 // exceed the shared memory's rate), two threads a row (213 against 197), output warps of their own, every fourth pair of
